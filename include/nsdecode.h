@@ -350,6 +350,16 @@ int nsd_ancestors(const uint8_t *backptr, int32_t t, int32_t N, int32_t B, uint8
 int nsd_add_rmsnorm(const void *x, const void *delta, const void *w, float eps, int32_t rows, int32_t hidden,
                     int32_t dtype, void *x_out, void *h, void *stream);
 
+/* Gradients of nsd_add_rmsnorm, for training through it (train_emg_llm.py:145-181): from the gradients dh of h and
+ * dx_out of x_out (NULL: x_out is not used elsewhere), with x_out as the forward stored it,
+ *   dx = dx_out + r (g - xh mean(g xh)),  r = rsqrt(mean(x_out^2) + eps), xh = x_out r, g = dh w:
+ * the gradient of x and of delta alike; dw (NULL: not wanted) = sum over the rows of dh xh.  Arrays in the element
+ * type, sums in fp32 and in a fixed order; the rounding of xh inside the forward is passed through.  dx may be dx_out
+ * or dh.  ws: nsd_add_rmsnorm_bwd_workspace bytes of device scratch, needed where dw is. */
+int64_t nsd_add_rmsnorm_bwd_workspace(int32_t rows, int32_t hidden);
+int nsd_add_rmsnorm_bwd(const void *x_out, const void *w, const void *dh, const void *dx_out, float eps, int32_t rows,
+                        int32_t hidden, int32_t dtype, void *dx, void *dw, void *ws, int64_t ws_bytes, void *stream);
+
 /* Rotary embedding (rotate-half form) of the q and k heads of qkv [M, (heads + 2 kv_heads) * hd] with the
  * step's cos / sin (fp32 [hd], both halves hold the same angles); q to q_out [M, heads, hd], k and v to the
  * step's slabs k_out / v_out [M, kv_heads, hd] of the generated cache. */
@@ -383,6 +393,51 @@ int nsd_attn_ctx(const void *q, const void *kctx_pad, const void *vctx_t, int32_
 /* out[r, i] = silu(gate_up[r, i]) * gate_up[r, inter + i]  (the SwiGLU between the two MLP contractions);
  * inter a multiple of 4 (fp32) / 8 (bf16). */
 int nsd_swiglu(const void *gate_up, int64_t rows, int32_t inter, int32_t dtype, void *out, void *stream);
+
+/* ---- attention of whole sequences, and of a beam over long shared prefixes ------------------------------------
+ * Shape of a call.  Query head hq reads kv head hq / (heads / kv_heads).  Strides count elements, in the order
+ * (batch, position, head); the hd elements of a row are consecutive.  Pointers and strides must be multiples of 16
+ * bytes, else NSD_E_ALIGN.  hd: a multiple of 8, 8 to 128; scale > 0; dtype 0 = fp32, 1 = bf16. */
+typedef struct NsdSeqAttn {
+    int32_t batch, len_q, len_k, heads, kv_heads, hd, dtype;
+    int32_t causal;                    /* query i sees keys j <= i + len_k - len_q (none for the first rows if len_q > len_k) */
+    float   scale;
+    int32_t reserved;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const uint8_t *key_mask;           /* device [batch, len_k] or NULL: 0 = no query sees this key; what its key and
+                                          value rows hold (NaN, Inf) takes no part in any result */
+    const int32_t *key_len;            /* device [batch] or NULL: keys at and after it are not seen (clamped to
+                                          [0, len_k]); not taken by nsd_attn_bwd */
+} NsdSeqAttn;
+
+/* out [batch, len_q, heads, hd] = softmax(scale q k^T over the visible keys) v; a row that sees no key is zeros.
+ *   lse  fp32 [batch, kv_heads, len_q, heads / kv_heads] or NULL: the natural logarithm of each row's sum of
+ *        exponentials (-inf for a row that sees no key), what nsd_attn_bwd recomputes the probabilities from
+ *   ws   device scratch of nsd_attn_fwd_workspace(p) bytes (may be NULL where that is 0), free again when the
+ *        stream has passed the call; NSD_E_SIZE if ws_bytes is less
+ * Results do not depend on anything but the arguments (no atomics; the split of the keys over workgroups is a
+ * function of the sizes).  Replaces the attention of the frozen LLM's layers (train_emg_llm.py:145-181). */
+int64_t nsd_attn_fwd_workspace(const NsdSeqAttn *p);
+int nsd_attn_fwd(const void *q, const void *k, const void *v, const NsdSeqAttn *p, void *out, float *lse,
+                 void *ws, int64_t ws_bytes, void *stream);
+
+/* Gradients of that attention for dout [batch, len_q, heads, hd]; out and lse as nsd_attn_fwd left them.
+ *   dq [batch, len_q, heads, hd], dk, dv [batch, len_k, kv_heads, hd] (summed over the query heads of a kv head);
+ *   zeros for masked keys and for rows that see no key.  ws: nsd_attn_bwd_workspace(p) bytes. */
+int64_t nsd_attn_bwd_workspace(const NsdSeqAttn *p);
+int nsd_attn_bwd(const void *q, const void *k, const void *v, const void *out, const float *lse, const void *dout,
+                 const NsdSeqAttn *p, void *dq, void *dk, void *dv, void *ws, int64_t ws_bytes, void *stream);
+
+/* Softmax state of a beam step over keys that hypotheses share, each key read once for all of them; any number of
+ * keys (nsd_attn_ctx holds at most 256).  Here batch counts the groups that share keys and len_q the hypotheses of a
+ * group: q [batch * len_q, heads, hd] (q_stride as for the other calls), k / v of group z at z * stride[0], position j,
+ * kv head h at j * stride[1] + h * stride[2]; causal = 0 and key_mask NULL; key_len for groups of differing lengths.
+ * Leaves part_o fp32 [batch * len_q * heads, hd], part_m / part_l fp32 [batch * len_q * heads] as nsd_attn_ctx does;
+ * with has_state != 0 they hold the state of other keys (another prefix level, nsd_attn_ctx), which is continued.
+ * nsd_attn_step continues it in turn.  ws: nsd_attn_prefix_workspace(p) bytes. */
+int64_t nsd_attn_prefix_workspace(const NsdSeqAttn *p);
+int nsd_attn_prefix(const void *q, const void *k, const void *v, const NsdSeqAttn *p, int32_t has_state,
+                    float *part_o, float *part_m, float *part_l, void *ws, int64_t ws_bytes, void *stream);
 
 /* Row-wise deterministic fp32 log-softmax, the one nsd_step applies
  * (F.log_softmax at scripts/ns_utils.py:227).  x, out device [rows, V]. */

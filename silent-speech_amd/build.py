@@ -15,8 +15,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 SO = PKG / "libnsdecode.so"
-SOURCES = ["nsd_step.hip", "nsd_aux.hip", "nsd_prior.hip", "nsd_attn.hip"]
-HEADERS = [CSRC / "nsd_device.h", ROOT / "include" / "nsdecode.h"]
+SOURCES = ["nsd_step.hip", "nsd_aux.hip", "nsd_prior.hip", "nsd_attn.hip", "nsd_seqattn.hip"]
+HEADERS = [CSRC / "nsd_device.h", CSRC / "nsd_elem.h", ROOT / "include" / "nsdecode.h"]
 FLAGS = ["-O3", "--offload-arch=gfx950", "-ffp-contract=off", "-fPIC", "-shared", "-std=c++17",
          "-fno-gpu-rdc", "-Wall", "-Wno-unused-function",
          # no packed fp32 instructions: some of their forms have given wrong results on these GPUs now and then

@@ -2,7 +2,7 @@
 // (inference_emg_llm.py:83-88) needs around its dense contractions when all N utterances x B hypotheses of a
 // beam step advance together and the generated keys / values are never moved:
 //   nsd_ancestors       hypothesis m's ancestor slot at every generated position, from the scorer's back-pointers
-//   nsd_add_rmsnorm     residual add + RMSNorm (one wave per row)
+//   nsd_add_rmsnorm     residual add + RMSNorm (one wave per row), nsd_add_rmsnorm_bwd its gradients
 //   nsd_rope_kv_append  rotary embedding of q and k, k / v written to the step's slab of the generated cache
 //   nsd_attn_step       attention of one new token per hypothesis over [context keys shared by the utterance ;
 //                       generated keys addressed through the ancestor table], online softmax, fp32 accumulation
@@ -11,74 +11,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "nsd_device.h"
+#include "nsd_elem.h"
 
 namespace {
-
-struct BF16 { uint16_t b; };
-
-template <class T> NSD_D float to_f(T v);
-template <> NSD_D float to_f<float>(float v) { return v; }
-template <> NSD_D float to_f<BF16>(BF16 v) { return __uint_as_float((uint32_t)v.b << 16); }
-
-template <class T> NSD_D T from_f(float v);
-template <> NSD_D float from_f<float>(float v) { return v; }
-template <> NSD_D BF16 from_f<BF16>(float v)
-{
-    uint32_t u = __float_as_uint(v);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return BF16{(uint16_t)((u >> 16) | 0x40u)};     // NaN stays NaN
-    u += 0x7fffu + ((u >> 16) & 1u);                                                   // round to nearest even
-    return BF16{(uint16_t)(u >> 16)};
-}
-
-// sixteen bytes of a row as floats: 4 (fp32) or 8 (bf16) elements
-template <class T> struct Vec16;
-template <> struct Vec16<float> {
-    static constexpr int N = 4;
-    NSD_D static void unpack(const uint4 &v, float (&o)[8])
-    {
-        o[0] = __uint_as_float(v.x); o[1] = __uint_as_float(v.y); o[2] = __uint_as_float(v.z); o[3] = __uint_as_float(v.w);
-    }
-    NSD_D static void load(const float *p, float (&o)[8]) { unpack(*reinterpret_cast<const uint4 *>(p), o); }
-};
-template <> struct Vec16<BF16> {
-    static constexpr int N = 8;
-    NSD_D static void unpack(const uint4 &v, float (&o)[8])
-    {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            o[2 * i] = __uint_as_float(w[i] << 16);
-            o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    }
-    NSD_D static void load(const BF16 *p, float (&o)[8]) { unpack(*reinterpret_cast<const uint4 *>(p), o); }
-};
-
-// Wave-wide maximum / sum, the same value in every lane.  Inside a row of 16 lanes the butterfly runs on DPP register
-// moves (after the distance-1 and -2 steps a quad is uniform, so the mirrored lane of the other quad / half carries
-// what the lane at distance 4 / 8 carries); the four row results meet through scalar registers.  No LDS-crossbar
-// permutes: they cost an address, an LDS instruction and its latency per step.
-NSD_D float nsd_dpp_row_mirror(float v)
-{
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, true));
-}
-NSD_D float row_lane(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
-NSD_D float wave_max_f(float v)
-{
-    v = fmaxf(v, nsd_dpp_xor1(v));
-    v = fmaxf(v, nsd_dpp_xor2(v));
-    v = fmaxf(v, nsd_dpp_half_mirror(v));
-    v = fmaxf(v, nsd_dpp_row_mirror(v));
-    return fmaxf(fmaxf(row_lane(v, 0), row_lane(v, 16)), fmaxf(row_lane(v, 32), row_lane(v, 48)));
-}
-NSD_D float wave_sum_f(float v)
-{
-    v = v + nsd_dpp_xor1(v);
-    v = v + nsd_dpp_xor2(v);
-    v = v + nsd_dpp_half_mirror(v);
-    v = v + nsd_dpp_row_mirror(v);
-    return (row_lane(v, 0) + row_lane(v, 16)) + (row_lane(v, 32) + row_lane(v, 48));
-}
 
 // ---------------------------------------------------------------------
 // ancestors: one wave per utterance, the utterance's back-pointers of steps 0..t-1 staged in LDS
@@ -104,20 +39,6 @@ nsd_ancestors_kernel(const uint8_t *backptr, int t, int M, int B, uint8_t *anc)
 // residual add + RMSNorm: x_out = x (+ delta); h = w * (x_out * rsqrt(mean(x_out^2) + eps)), one wave per row,
 // sixteen bytes per lane and access (hidden must be a multiple of the 4 / 8 elements that makes)
 // ---------------------------------------------------------------------
-template <class T> struct Store16;
-template <> struct Store16<float> {
-    NSD_D static void store(float *p, const float (&v)[8]) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-};
-template <> struct Store16<BF16> {
-    NSD_D static void store(BF16 *p, const float (&v)[8])
-    {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)from_f<BF16>(v[2 * i]).b | ((uint32_t)from_f<BF16>(v[2 * i + 1]).b << 16);
-        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-};
-
 template <class T>
 __global__ void __launch_bounds__(256)
 nsd_add_rmsnorm_kernel(const T *x, const T *delta, const T *w, float eps, int rows, int hidden, T *x_out, T *h)
@@ -220,6 +141,200 @@ void launch_add_rmsnorm(const T *x, const T *delta, const T *w, float eps, int r
     else
         hipLaunchKernelGGL(nsd_add_rmsnorm_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s,
                            x, delta, w, eps, rows, hidden, x_out, h);
+}
+
+// ---------------------------------------------------------------------
+// backward of residual add + RMSNorm.  With r = rsqrt(mean(x^2) + eps), xh = x r and g = dh w:
+//   dx = dx_out + r (g - xh mean(g xh)) = dx_out + r g - x r^3 mean(g x),   dw = sum over the rows of dh xh.
+// Both row sums are taken in one pass.  A workgroup holds a row in registers as the forward does, and walks over rows
+// blockIdx.x, + gridDim.x, ...: a thread then meets the same columns in every row and keeps their part of dw in
+// registers; the workgroups' parts (fp32) are summed in a fixed order by nsd_colsum_kernel.
+// ---------------------------------------------------------------------
+template <class T, int NV>
+__global__ void __launch_bounds__(1024)
+nsd_add_rmsnorm_bwd_kernel(const T *x, const T *w, const T *dh, const T *dx_out, float eps, int rows, int hidden, T *dx,
+                           float *dw_part)
+{
+    constexpr int VN = Vec16<T>::N;
+    __shared__ float part[2][2][16];
+    const int nvec = hidden / VN, waves = (int)blockDim.x >> 6;
+    float wv[NV][8], dw[NV][8];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int i = (int)threadIdx.x + k * (int)blockDim.x;
+#pragma unroll
+        for (int e = 0; e < VN; ++e) dw[k][e] = 0.0f;
+        if (i < nvec) Vec16<T>::load(w + (size_t)i * VN, wv[k]);
+    }
+    int buf = 0;
+    for (int row = blockIdx.x; row < rows; row += gridDim.x, buf ^= 1) {
+        const size_t base = (size_t)row * hidden;
+        float xv[NV][8], gv[NV][8], ov[NV][8];
+        float ss = 0.0f, gx = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int i = (int)threadIdx.x + k * (int)blockDim.x;
+            if (i < nvec) {
+                Vec16<T>::load(x + base + (size_t)i * VN, xv[k]);
+                Vec16<T>::load(dh + base + (size_t)i * VN, gv[k]);
+                if (dx_out) Vec16<T>::load(dx_out + base + (size_t)i * VN, ov[k]);
+#pragma unroll
+                for (int e = 0; e < VN; ++e) {
+                    ss = __builtin_fmaf(xv[k][e], xv[k][e], ss);
+                    gx = __builtin_fmaf(gv[k][e] * wv[k][e], xv[k][e], gx);
+                }
+            }
+        }
+        ss = wave_sum_f(ss);
+        gx = wave_sum_f(gx);
+        if ((threadIdx.x & 63) == 0) {
+            part[buf][0][threadIdx.x >> 6] = ss;
+            part[buf][1][threadIdx.x >> 6] = gx;
+        }
+        __syncthreads();                                        // (the other half of `part` is free until the next one)
+        ss = gx = 0.0f;
+        for (int q = 0; q < waves; ++q) { ss += part[buf][0][q]; gx += part[buf][1][q]; }
+        const float r = rsqrtf(ss / (float)hidden + eps);
+        const float c = r * r * r * (gx / (float)hidden);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int i = (int)threadIdx.x + k * (int)blockDim.x;
+            if (i < nvec) {
+#pragma unroll
+                for (int e = 0; e < VN; ++e) {
+                    dw[k][e] = __builtin_fmaf(gv[k][e], xv[k][e] * r, dw[k][e]);
+                    const float d = __builtin_fmaf(gv[k][e] * wv[k][e], r, -(xv[k][e] * c));
+                    xv[k][e] = dx_out ? ov[k][e] + d : d;
+                }
+                Store16<T>::store(dx + base + (size_t)i * VN, xv[k]);
+            }
+        }
+    }
+    if (dw_part) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int i = (int)threadIdx.x + k * (int)blockDim.x;
+            if (i < nvec) {
+                float *p = dw_part + (size_t)blockIdx.x * hidden + (size_t)i * VN;
+#pragma unroll
+                for (int e = 0; e < VN; ++e) p[e] = dw[k][e];
+            }
+        }
+    }
+}
+
+// Rows that no workgroup can hold in registers: the row is read twice, r is left for the second kernel, whose threads
+// own columns and walk over the rows blockIdx.y, + gridDim.y, ...
+template <class T>
+__global__ void __launch_bounds__(1024)
+nsd_add_rmsnorm_bwd_long_kernel(const T *x, const T *w, const T *dh, const T *dx_out, float eps, int hidden, T *dx, float *rs)
+{
+    constexpr int VN = Vec16<T>::N;
+    __shared__ float part[2][16];
+    const size_t base = (size_t)blockIdx.x * hidden;
+    float ss = 0.0f, gx = 0.0f;
+    for (int i = (int)threadIdx.x * VN; i < hidden; i += (int)blockDim.x * VN) {
+        float xv[8], gv[8], wv[8];
+        Vec16<T>::load(x + base + i, xv);
+        Vec16<T>::load(dh + base + i, gv);
+        Vec16<T>::load(w + i, wv);
+#pragma unroll
+        for (int e = 0; e < VN; ++e) {
+            ss = __builtin_fmaf(xv[e], xv[e], ss);
+            gx = __builtin_fmaf(gv[e] * wv[e], xv[e], gx);
+        }
+    }
+    ss = wave_sum_f(ss);
+    gx = wave_sum_f(gx);
+    if ((threadIdx.x & 63) == 0) {
+        part[0][threadIdx.x >> 6] = ss;
+        part[1][threadIdx.x >> 6] = gx;
+    }
+    __syncthreads();
+    ss = gx = 0.0f;
+    for (int q = 0; q < (int)(blockDim.x >> 6); ++q) { ss += part[0][q]; gx += part[1][q]; }
+    const float r = rsqrtf(ss / (float)hidden + eps);
+    const float c = r * r * r * (gx / (float)hidden);
+    for (int i = (int)threadIdx.x * VN; i < hidden; i += (int)blockDim.x * VN) {
+        float xv[8], gv[8], wv[8], ov[8];
+        Vec16<T>::load(x + base + i, xv);
+        Vec16<T>::load(dh + base + i, gv);
+        Vec16<T>::load(w + i, wv);
+        if (dx_out) Vec16<T>::load(dx_out + base + i, ov);
+#pragma unroll
+        for (int e = 0; e < VN; ++e) {
+            const float d = __builtin_fmaf(gv[e] * wv[e], r, -(xv[e] * c));
+            xv[e] = dx_out ? ov[e] + d : d;
+        }
+        Store16<T>::store(dx + base + i, xv);
+    }
+    if (rs && threadIdx.x == 0) rs[blockIdx.x] = r;
+}
+
+template <class T>
+__global__ void __launch_bounds__(256)
+nsd_rmsnorm_dw_kernel(const T *x, const T *dh, const float *rs, int rows, int hidden, float *dw_part)
+{
+    constexpr int VN = Vec16<T>::N;
+    const int i = (int)(blockIdx.x * blockDim.x + threadIdx.x) * VN;
+    if (i >= hidden) return;
+    float dw[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+        float xv[8], gv[8];
+        Vec16<T>::load(x + (size_t)row * hidden + i, xv);
+        Vec16<T>::load(dh + (size_t)row * hidden + i, gv);
+        const float r = rs[row];
+#pragma unroll
+        for (int e = 0; e < VN; ++e) dw[e] = __builtin_fmaf(gv[e], xv[e] * r, dw[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < VN; ++e) dw_part[(size_t)blockIdx.y * hidden + i + e] = dw[e];
+}
+
+// out[c] = sum over n rows of part[:, c]: 64 columns for each workgroup, its four waves take every fourth row
+template <class T>
+__global__ void __launch_bounds__(256)
+nsd_colsum_kernel(const float *part, int n, int hidden, T *out)
+{
+    __shared__ float s[4][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = (int)blockIdx.x * 64 + lane;
+    float a = 0.0f, b = 0.0f;
+    if (c < hidden) {
+        int r = w;
+        for (; r + 4 < n; r += 8) {
+            a += part[(size_t)r * hidden + c];
+            b += part[(size_t)(r + 4) * hidden + c];
+        }
+        if (r < n) a += part[(size_t)r * hidden + c];
+    }
+    s[w][lane] = a + b;
+    __syncthreads();
+    if (w == 0 && c < hidden) out[c] = from_f<T>((s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]));
+}
+
+// workgroups of the backward pass (rows of its partial sums of dw)
+int norm_bwd_parts(int rows) { return rows < 512 ? rows : 512; }
+
+template <class T>
+int launch_add_rmsnorm_bwd(const T *x, const T *w, const T *dh, const T *dx_out, float eps, int rows, int hidden, T *dx, T *dw,
+                           float *ws, hipStream_t s)
+{
+    constexpr int VN = Vec16<T>::N, NV = 2;
+    const int nvec = hidden / VN, waves = (nvec + 64 * NV - 1) / (64 * NV), parts = norm_bwd_parts(rows);
+    if (waves <= 16) {
+        hipLaunchKernelGGL((nsd_add_rmsnorm_bwd_kernel<T, NV>), dim3((unsigned)parts), dim3(64 * waves), 0, s,
+                           x, w, dh, dx_out, eps, rows, hidden, dx, dw ? ws : nullptr);
+    } else {
+        float *rs = dw ? ws + (size_t)parts * hidden : nullptr;
+        hipLaunchKernelGGL(nsd_add_rmsnorm_bwd_long_kernel<T>, dim3((unsigned)rows), dim3(1024), 0, s,
+                           x, w, dh, dx_out, eps, hidden, dx, rs);
+        if (dw)
+            hipLaunchKernelGGL(nsd_rmsnorm_dw_kernel<T>, dim3((unsigned)((nvec + 255) / 256), (unsigned)parts), dim3(256), 0, s,
+                               x, dh, rs, rows, hidden, ws);
+    }
+    if (dw)
+        hipLaunchKernelGGL(nsd_colsum_kernel<T>, dim3((unsigned)((hidden + 63) / 64)), dim3(256), 0, s, ws, parts, hidden, dw);
+    return (int)hipGetLastError();
 }
 
 // ---------------------------------------------------------------------
@@ -709,6 +824,33 @@ extern "C" int nsd_add_rmsnorm(const void *x, const void *delta, const void *w, 
         launch_add_rmsnorm<BF16>((const BF16 *)x, (const BF16 *)delta, (const BF16 *)w, eps, rows, hidden,
                                  (BF16 *)x_out, (BF16 *)h, (hipStream_t)stream);
     return (int)hipGetLastError();
+}
+
+extern "C" int64_t nsd_add_rmsnorm_bwd_workspace(int32_t rows, int32_t hidden)
+{
+    if (rows < 1 || hidden < 1) return 0;
+    return ((int64_t)norm_bwd_parts(rows) * hidden + rows) * 4;
+}
+
+extern "C" int nsd_add_rmsnorm_bwd(const void *x_out, const void *w, const void *dh, const void *dx_out, float eps, int32_t rows,
+                                   int32_t hidden, int32_t dtype, void *dx, void *dw, void *ws, int64_t ws_bytes, void *stream)
+{
+    if (rows < 0 || hidden < 1 || (dtype != 0 && dtype != 1) || hidden % (dtype ? 8 : 4)) return NSD_E_SIZE;
+    if (rows == 0 && !dw) return NSD_OK;
+    if ((rows > 0 && (!x_out || !w || !dh || !dx)) || (rows > 0 && dw && !ws)) return NSD_E_NULL;
+    if (!aligned16(x_out, w, dh, dx_out, dx, dw, ws)) return NSD_E_ALIGN;
+    if (dw && ws_bytes < nsd_add_rmsnorm_bwd_workspace(rows, hidden)) return NSD_E_SIZE;
+    if (rows == 0) {                                            // a sum over no rows
+        const dim3 grid((unsigned)((hidden + 63) / 64)), block(256);
+        if (dtype == 0) hipLaunchKernelGGL(nsd_colsum_kernel<float>, grid, block, 0, (hipStream_t)stream, nullptr, 0, hidden, (float *)dw);
+        else hipLaunchKernelGGL(nsd_colsum_kernel<BF16>, grid, block, 0, (hipStream_t)stream, nullptr, 0, hidden, (BF16 *)dw);
+        return (int)hipGetLastError();
+    }
+    if (dtype == 0)
+        return launch_add_rmsnorm_bwd<float>((const float *)x_out, (const float *)w, (const float *)dh, (const float *)dx_out, eps,
+                                             rows, hidden, (float *)dx, (float *)dw, (float *)ws, (hipStream_t)stream);
+    return launch_add_rmsnorm_bwd<BF16>((const BF16 *)x_out, (const BF16 *)w, (const BF16 *)dh, (const BF16 *)dx_out, eps, rows,
+                                        hidden, (BF16 *)dx, (BF16 *)dw, (float *)ws, (hipStream_t)stream);
 }
 
 extern "C" int nsd_rope_kv_append(const void *qkv, const float *cos_t, const float *sin_t, int32_t M, int32_t heads,

@@ -53,12 +53,22 @@ class BeamStatePtrs(C.Structure):
                 ("meta", C.c_void_p), ("utt", C.c_void_p), ("done_count", C.c_void_p)]
 
 
+class SeqAttn(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("len_q", C.c_int32), ("len_k", C.c_int32), ("heads", C.c_int32),
+                ("kv_heads", C.c_int32), ("hd", C.c_int32), ("dtype", C.c_int32), ("causal", C.c_int32),
+                ("scale", C.c_float), ("reserved", C.c_int32), ("q_stride", C.c_int64 * 3),
+                ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("key_mask", C.c_void_p),
+                ("key_len", C.c_void_p)]
+
+
 EXPORTS = ["nsd_version", "nsd_strerror", "nsd_hash64", "nsd_tables_create", "nsd_tables_destroy",
            "nsd_tables_order", "nsd_state_init", "nsd_step", "nsd_backtrace", "nsd_gather_ids",
            "nsd_ctc_greedy", "nsd_lm_logp", "nsd_rerank_gather", "nsd_log_softmax", "nsd_synth_logits",
            "nsd_decode_synth", "nsd_rerank_lm", "nsd_cond_dist", "nsd_lm_prior_ce", "nsd_lm_prior_ce_grad", "nsd_kv_reorder",
            "nsd_shutdown", "nsd_decode_synth_noalloc", "nsd_ancestors", "nsd_add_rmsnorm", "nsd_rope_kv_append",
-           "nsd_attn_step", "nsd_attn_ctx", "nsd_swiglu"]
+           "nsd_attn_step", "nsd_attn_ctx", "nsd_swiglu", "nsd_add_rmsnorm_bwd", "nsd_add_rmsnorm_bwd_workspace",
+           "nsd_attn_fwd", "nsd_attn_fwd_workspace", "nsd_attn_bwd", "nsd_attn_bwd_workspace", "nsd_attn_prefix",
+           "nsd_attn_prefix_workspace"]
 
 _lib = None
 
@@ -107,6 +117,15 @@ def load():
     L.nsd_cond_dist.argtypes = [vp, vp, vp, i32, i32, i32, vp, vp]
     L.nsd_lm_prior_ce.argtypes = [vp, vp, vp, i32, i32, i32, i32, vp, vp, vp]
     L.nsd_lm_prior_ce_grad.argtypes = [vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp]
+    L.nsd_add_rmsnorm_bwd_workspace.restype = i64
+    L.nsd_add_rmsnorm_bwd_workspace.argtypes = [i32, i32]
+    L.nsd_add_rmsnorm_bwd.argtypes = [vp, vp, vp, vp, C.c_float, i32, i32, i32, vp, vp, vp, i64, vp]
+    for name in ("nsd_attn_fwd_workspace", "nsd_attn_bwd_workspace", "nsd_attn_prefix_workspace"):
+        getattr(L, name).restype = i64
+        getattr(L, name).argtypes = [C.POINTER(SeqAttn)]
+    L.nsd_attn_fwd.argtypes = [vp, vp, vp, C.POINTER(SeqAttn), vp, vp, vp, i64, vp]
+    L.nsd_attn_bwd.argtypes = [vp, vp, vp, vp, vp, vp, C.POINTER(SeqAttn), vp, vp, vp, vp, i64, vp]
+    L.nsd_attn_prefix.argtypes = [vp, vp, vp, C.POINTER(SeqAttn), i32, vp, vp, vp, vp, i64, vp]
     for name in EXPORTS:
         getattr(L, name)
     _lib = L
