@@ -74,27 +74,34 @@ NSD_D float half_sum(float v)
 }
 NSD_D float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
 
-// A tile of rows in LDS, DP elements each, in 16-byte pieces.  Piece p of row r lies at p ^ sw(r): eight lanes that
-// read the same piece of eight rows (the operand reads along a row) and sixteen lanes that read 32 bytes of four rows
-// (the transposing reads) then touch every bank once.
+// A tile of rows in LDS, DP elements each, in 16-byte pieces, as chunks of 16 rows x 4 pieces (1 KiB, what a wave fetches
+// with one instruction, 64 bytes of a row by four adjacent lanes).  Piece p of row r lies at place p ^ g(r) of its row's
+// four: sixteen lanes that read one piece of sixteen rows (the operand reads along a row) touch all 64 banks once, and so
+// do the 32 lanes that read 32 bytes of eight rows (the transposing reads).  Whole chunks are a constant apart, so an
+// operand's many reads are few address registers and immediate offsets (with a swizzle across the whole row every one
+// had an address of its own: 20 registers, which the kernels' two waves per SIMD do not have).
 template <class T, int DP> struct Tile {
     static constexpr int RB = DP * (int)sizeof(T);              // bytes of a row
     static constexpr int PR = RB / 16;                          // pieces of a row
+    static constexpr int CG = PR / 4;                           // chunks of 16 rows
     static constexpr bool B16 = sizeof(T) == 2;
-    NSD_D static int sw(int row) { return !B16 ? row & 7 : DP == 128 ? (row & 7) << 1 : (row >> 1 & 3) << 1; }
-    NSD_D static int at(int row, int piece) { return row * RB + ((piece ^ sw(row)) << 4); }
+    NSD_D static int g(int r) { return (r >> 1 & 3) ^ (r >> 3 & 1); }
 
-    // elements 16 kc + 8 h .. + 7 of row `row` (h = lane half)
-    NSD_D static Frag<T> row_frag(const char *s, int row, int kc, int h)
+    // elements 16 kc + 8 h .. + 7 of row row0 + c32 (row0 a multiple of 32; lane = 32 h + c32)
+    NSD_D static Frag<T> row_frag(const char *s, int row0, int kc, int lane)
     {
         Frag<T> f;
+        const int c32 = lane & 31, h = lane >> 5, r = c32 & 15;
+        const char *p = s + ((row0 >> 4) + (c32 >> 4)) * (CG * 1024) + r * 64;
         if constexpr (B16) {
-            f.v = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4 *>(s + at(row, 2 * kc + h)));
+            const int x = ((h ^ g(r)) << 4) ^ ((kc & 1) << 5);
+            f.v = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4 *>(p + x + (kc >> 1) * 1024));
         } else {
-            const float4 x = *reinterpret_cast<const float4 *>(s + at(row, 4 * kc + 2 * h));
-            const float4 y = *reinterpret_cast<const float4 *>(s + at(row, 4 * kc + 2 * h + 1));
-            f.v[0] = x.x; f.v[1] = x.y; f.v[2] = x.z; f.v[3] = x.w;
-            f.v[4] = y.x; f.v[5] = y.y; f.v[6] = y.z; f.v[7] = y.w;
+            const int x = (2 * h ^ g(r)) << 4;
+            const float4 u = *reinterpret_cast<const float4 *>(p + x + kc * 1024);
+            const float4 v = *reinterpret_cast<const float4 *>(p + (x ^ 16) + kc * 1024);
+            f.v[0] = u.x; f.v[1] = u.y; f.v[2] = u.z; f.v[3] = u.w;
+            f.v[4] = v.x; f.v[5] = v.y; f.v[6] = v.z; f.v[7] = v.w;
         }
         return f;
     }
@@ -103,20 +110,21 @@ template <class T, int DP> struct Tile {
     {
         Frag<T> f;
         const int h = lane >> 5;
+        const char *p = s + (r0 >> 4) * (CG * 1024);
         if constexpr (B16) {
             // sixteen lanes hand in 32 bytes of four rows and get a column of sixteen each
-            const int row = r0 + 4 * h + (lane >> 2 & 3);
-            const char *p = s + at(row, 4 * dt + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) + 8 * (lane & 1);
+            const int r = 4 * h + (lane >> 2 & 3), piece = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
+            const int x = ((piece ^ g(r)) << 4) + 8 * (lane & 1);
             typedef __attribute__((address_space(3))) s16x4 lds4;
-            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)p);
-            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + 8 * RB));
-            f.v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + r * 64 + x + dt * 1024));
+            const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + r * 64 + (x ^ 16) + 512 + dt * 1024));
+            f.v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
-            const int d = 32 * dt + (lane & 31);
+            const int piece = lane >> 2 & 3;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int row = r0 + 8 * (j >> 2) + 4 * h + (j & 3);
-                f.v[j] = *reinterpret_cast<const float *>(s + at(row, d >> 2) + 4 * (d & 3));
+                const int r = 8 * (j >> 2) + 4 * h + (j & 3);
+                f.v[j] = *reinterpret_cast<const float *>(p + (2 * dt + (lane >> 4 & 1)) * 1024 + r * 64 + ((piece ^ g(r)) << 4) + 4 * (lane & 3));
             }
         }
         return f;
@@ -166,6 +174,90 @@ NSD_D void store4(BF16 *p, float a, float b, float c, float d)
     *reinterpret_cast<uint2 *>(p) = make_uint2(u, w);
 }
 
+// What rounding to bf16 took from v, in 256ths of the last place that bf16 keeps: a signed byte, with which the row sums
+// dO . O of the backward pass see 16 bits of O.  (With bf16's 8 alone the error of dQ and dK grows by up to 1.3 times, at
+// short rows; the whole rest in bf16 costs 13 us of traffic in a training step of 8 x 640 positions, the byte half of it.)
+NSD_D float pow2_of(BF16 v) { return __uint_as_float((uint32_t)(v.b & 0x7f80u) << 16); }
+NSD_D int rest_of(float v)
+{
+    const BF16 r = from_f<BF16>(v);
+    const float inv = __uint_as_float(0x7f000000u - ((uint32_t)(r.b & 0x7f80u) << 16));
+    return (int)fminf(fmaxf(__builtin_rintf((v - to_f(r)) * inv * 32768.0f), -127.0f), 127.0f);
+}
+NSD_D uint32_t rest4(float a, float b, float c, float d)
+{
+    return (uint32_t)(rest_of(a) & 255) | (uint32_t)(rest_of(b) & 255) << 8 | (uint32_t)(rest_of(c) & 255) << 16 | (uint32_t)rest_of(d) << 24;
+}
+// sum of g times the rest of o over a lane's eight elements
+NSD_D float rest_dot(const Frag<BF16> &g, const Frag<BF16> &o, const int8_t *rest, float s)
+{
+    const uint2 c = *reinterpret_cast<const uint2 *>(rest);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int8_t b = (int8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
+        const float f = pow2_of(__builtin_bit_cast(BF16, (__bf16)o.v[j]));
+        s = __builtin_fmaf((float)g.v[j], (float)b * f * (1.0f / 32768.0f), s);
+    }
+    return s;
+}
+NSD_D float rest_dot(const Frag<float> &, const Frag<float> &, const int8_t *, float s) { return s; }
+
+// A wave's 32 rows from its transposed accumulators (lane = row, registers = elements) to memory, times `mul`.  bf16 rows
+// pass through LDS (`s`, the wave's own 32 * (RB + 16) bytes) and leave in 16-byte pieces of whole rows: stored from the
+// accumulators they would be 8 bytes here and there, 16 stores that touch 32 rows each.  ptr(r) is row r's place or null.
+template <class T, int DP, class P>
+NSD_D void put_rows(char *s, const f32x16 (&o)[DP / 32], float mul, int D, int lane, P ptr)
+{
+    const int c32 = lane & 31, h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+        constexpr int PR = DP / 8, SB = DP * 2 + 16;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                store4(reinterpret_cast<T *>(s + c32 * SB) + 32 * dt + 8 * b + 4 * h, o[dt][4 * b] * mul, o[dt][4 * b + 1] * mul,
+                       o[dt][4 * b + 2] * mul, o[dt][4 * b + 3] * mul);
+        nsd_wave_sync();
+#pragma unroll
+        for (int i = 0; i < 32 * PR / 64; ++i) {
+            const int r = (i * 64 + lane) / PR, p = (i * 64 + lane) % PR;
+            T *dst = ptr(r);
+            if (dst && p * 8 < D) *reinterpret_cast<uint4 *>(dst + p * 8) = *reinterpret_cast<const uint4 *>(s + r * SB + p * 16);
+        }
+        nsd_wave_sync();
+    } else {
+        T *dst = ptr(c32);
+        if (!dst) return;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int d = 32 * dt + 8 * b + 4 * h;
+                if (d < D) store4(dst + d, o[dt][4 * b] * mul, o[dt][4 * b + 1] * mul, o[dt][4 * b + 2] * mul, o[dt][4 * b + 3] * mul);
+            }
+    }
+}
+// The rows' rests, a byte an element, the same way (bf16 only).
+template <int DP, class P>
+NSD_D void put_rest(char *s, const f32x16 (&o)[DP / 32], float mul, int D, int lane, P ptr)
+{
+    const int c32 = lane & 31, h = lane >> 5;
+    constexpr int PR = DP / 8, SB = DP + 16;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            *reinterpret_cast<uint32_t *>(s + c32 * SB + 32 * dt + 8 * b + 4 * h) =
+                rest4(o[dt][4 * b] * mul, o[dt][4 * b + 1] * mul, o[dt][4 * b + 2] * mul, o[dt][4 * b + 3] * mul);
+    nsd_wave_sync();
+#pragma unroll
+    for (int i = 0; i < 32 * PR / 64; ++i) {
+        const int r = (i * 64 + lane) / PR, p = (i * 64 + lane) % PR;
+        int8_t *dst = ptr(r);
+        if (dst && p * 8 < D) *reinterpret_cast<uint2 *>(dst + p * 8) = *reinterpret_cast<const uint2 *>(s + r * SB + p * 8);
+    }
+}
+
 // ---------------------------------------------------------------------
 // arguments.  Strides count elements; rows rho = i * G + g of a (z, kv head) pair, R = Lq * G of them.
 // ---------------------------------------------------------------------
@@ -180,47 +272,111 @@ struct SeqArgs {
     // forward
     void *out;                             // [Z, Lq, heads, D]
     float *lse;                            // [Z, KVH, R], natural logarithm
+    int8_t *rest;                          // a byte for each element of out, or null: see rest_of
     float *po, *pm, *pl;                   // state [splits][Z * Lq * heads] (sum of weighted values, maximum, sum)
     const float *in_o, *in_m, *in_l;       // a state to continue, or null
-    int splits, split_tiles;
+    int splits, split_tiles, batch;
     // backward
     const void *dout;                      // [Z, Lq, heads, D]
     float *delta;                          // [Z, KVH, R]
     void *dq, *dk, *dv;                    // contiguous like q, k, v
+    float *part, *part_v;                  // splits > 1: fp32 sums of dq, or of dk and dv, [splits] of them
     float scale;
 };
 
 NSD_D int div_g(int rho, uint32_t magic, int G) { return G == 1 ? rho : (int)(((uint64_t)(uint32_t)rho * magic) >> 32); }
 
-// the 64 (or fewer) keys from j0 on that exist and are not masked, as a word that every lane has
-NSD_D uint64_t key_word(const SeqArgs &a, const uint8_t *mask, int j0, int n_keys)
+// Work of a workgroup: which of `tiles` of which of `pairs` (batch, kv head and split of its keys).  Workgroups go to the
+// eight XCDs in turn, each with an L2 of its own: where the pairs divide evenly every XCD takes whole pairs, so that the
+// tiles of a pair share its L2, `batch` pairs at a time (enough to fill the XCD), and among those the costly tiles first.
+NSD_D void work_of(int bid, int tiles, int pairs, int batch, int &pair, int &tile)
 {
-    const int j = j0 + (int)(threadIdx.x & 63);
-    bool ok = j < n_keys;
-    if (mask && ok) ok = mask[j] != 0;
-    return __ballot(ok);
+    const int xcds = pairs % 8 == 0 ? 8 : 1, per = pairs / xcds;
+    const int x = bid % xcds, i = bid / xcds;
+    const int first = i / (batch * tiles) * batch, n = min(batch, per - first), j = i - first * tiles;
+    pair = (first + j % n) * xcds + x;
+    tile = j / n;
 }
 
-// One tile of ROWS rows on its way from memory to LDS, 256 threads: U pieces of 16 bytes for each.
-template <class T, int DP, int ROWS> struct Stage {
-    static constexpr int PR = Tile<T, DP>::PR, U = ROWS * PR / 256, EP = 16 / (int)sizeof(T);
-    uint4 x[U];
-    // rows row0 .. of a matrix at `base` with `stride` elements between rows; row r is there if ok(r)
-    template <class F> NSD_D void load(const T *base, int64_t stride, int D, F ok)
+// The keys of a tile that exist and are not masked, as words that every lane has.  A lane asks for its key's mask byte a
+// tile before the word is needed, so that no tile waits for it.
+template <int NW> struct KeyMask {
+    const uint8_t *mask;
+    int n_keys;
+    uint32_t byte[NW];
+    NSD_D void ask(int j0)
     {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = (int)threadIdx.x + 256 * u, r = i / PR, p = i % PR;
-            x[u] = make_uint4(0, 0, 0, 0);
-            if (p * EP < D && ok(r)) x[u] = *reinterpret_cast<const uint4 *>(base + r * stride + p * EP);
+        for (int i = 0; i < NW; ++i) {
+            const int j = j0 + 64 * i + (int)(threadIdx.x & 63);
+            byte[i] = j < n_keys ? 1 : 0;
+            if (mask && j < n_keys) byte[i] = mask[j];
         }
     }
-    NSD_D void put(char *s) const
+    // (a tile of 32 keys uses the lower half of its word)
+    NSD_D bool words(uint64_t (&w)[NW], uint64_t part) const
     {
+        uint64_t any = 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) any |= w[i] = __ballot(byte[i] != 0) & part;
+        return any != 0;
+    }
+};
+
+// A tile of ROWS rows goes from memory straight to LDS (global_load_lds), 16 bytes a lane and instruction: a wave fills
+// 1 KiB in lane order, so the piece that a lane fetches is the one that the swizzle puts at its place.  Rows that are
+// not there, and pieces past a row's D elements, come from a page of zeros: no query may see what lies there, not even
+// as 0 * NaN.  The load is written out because the compiler, which cannot tell the two halves of the double buffer
+// apart, would wait for it before the next transposing read of the other half; tile_barrier() is the wait.
+__device__ const uint4 zero_page[1] = {};
+
+NSD_D void to_lds(uint64_t g, uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(g), "s"(lds) : "memory");
+}
+// every wave's loads have arrived, and every wave is done with what they will overwrite next
+NSD_D void tile_barrier()
+{
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    __syncthreads();
+}
+NSD_D uint32_t lds_at(const char *p)
+{
+    typedef __attribute__((address_space(3))) const char lds_char;
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char *)p);
+}
+
+// This lane's part of a tile of ROWS rows: the wave fetches chunks w + 4 u, of which the lane fetches one piece.
+template <class T, int DP, int ROWS> struct Stage {
+    static constexpr int CG = Tile<T, DP>::CG, U = ROWS / 16 * CG / 4, EP = 16 / (int)sizeof(T);
+    int w, row, elem;                                           // row in a chunk, element in a chunk's rows
+    NSD_D Stage()
+    {
+        const int lane = threadIdx.x & 63;
+        w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        row = lane >> 2;
+        elem = ((lane & 3) ^ Tile<T, DP>::g(row)) * EP;
+    }
+    NSD_D int chunk_row(int u) const { return (w + 4 * u) / CG * 16; }
+    NSD_D int chunk_elem(int u) const { return (w + 4 * u) % CG * 4 * EP; }
+    NSD_D uint32_t place(uint32_t tile, int u) const { return tile + (w + 4 * u) * 1024; }
+    // rows of `base`, `stride` elements apart; row r of the tile is there if bit r of `words` is set
+    template <int NW> NSD_D void load(const T *base, int64_t stride, int D, const uint64_t (&words)[NW], const char *tile) const
+    {
+        const uint64_t p = (uint64_t)(base + row * stride + elem), zero = (uint64_t)zero_page;
+        const uint32_t dst = lds_at(tile);
+        bool whole = D == DP;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) whole = whole && words[i] == (ROWS < 64 ? (1ull << (ROWS & 63)) - 1 : ~0ull);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = (int)threadIdx.x + 256 * u;
-            *reinterpret_cast<uint4 *>(s + Tile<T, DP>::at(i / PR, i % PR)) = x[u];
+            uint64_t q = p + (uint64_t)(chunk_row(u) * stride + chunk_elem(u)) * sizeof(T);
+            if (!whole) {
+                const int r = chunk_row(u) + row;
+                const bool ok = chunk_elem(u) + elem < D && (words[NW > 1 ? r >> 6 : 0] >> (r & 63) & 1);
+                q = ok ? q : zero;
+            }
+            to_lds(q, place(dst, u));
         }
     }
 };
@@ -230,7 +386,7 @@ template <class T, int DP, int ROWS> struct Stage {
 // BN = KW * WN each; their states meet at the end).  grid.x = row tile, (z, kv head), split.
 // ---------------------------------------------------------------------
 template <class T, int DP, int WM, int KW, int NBUF, bool STATE>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && NBUF * KW / WM * DP <= 4096 ? 2 : 1)
 nsd_attn_fwd_kernel(SeqArgs a)
 {
     constexpr int WN = 4 / WM, BM = 32 * WM, BN = KW * WN, NK = KW / 32, DT = DP / 32, KC = DP / 16;
@@ -244,13 +400,10 @@ nsd_attn_fwd_kernel(SeqArgs a)
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c32 = lane & 31;
     const int wm = w % WM, wn = w / WM;
     const int rtiles = (a.R + BM - 1) / BM;
-    int bid = blockIdx.x;
-    const int split = bid % a.splits;
-    bid /= a.splits;
-    // later rows of a causal mask see more keys: their tiles start first
-    const int rt = rtiles - 1 - bid % rtiles;
-    bid /= rtiles;
-    const int kvh = bid % a.KVH, z = bid / a.KVH;
+    int pair, tile;
+    work_of(blockIdx.x, rtiles, a.Z * a.KVH * a.splits, a.batch, pair, tile);
+    const int rt = rtiles - 1 - tile;                           // later rows of a causal mask see more keys
+    const int split = pair % a.splits, kvh = pair / a.splits % a.KVH, z = pair / a.splits / a.KVH;
     const int n_keys = a.lens ? min(max(a.lens[z], 0), a.Lk) : a.Lk;
     const uint8_t *mask = a.mask ? a.mask + (size_t)z * a.Lk : nullptr;
 
@@ -267,6 +420,9 @@ nsd_attn_fwd_kernel(SeqArgs a)
 
     const T *kb = static_cast<const T *>(a.k) + z * a.k_sz + kvh * a.k_sh;
     const T *vb = static_cast<const T *>(a.v) + z * a.v_sz + kvh * a.v_sh;
+    constexpr uint64_t PART = BN < 64 ? (1ull << (BN & 63)) - 1 : ~0ull;
+    KeyMask<NW> keys{mask, n_keys, {}};
+    if (t < t_end) keys.ask(t * BN);
     Frag<T> qf[KC];
     {
         const T *qp = static_cast<const T *>(a.q) + z * a.q_sz + i_row * a.q_st + head * a.q_sh;
@@ -297,27 +453,31 @@ nsd_attn_fwd_kernel(SeqArgs a)
         }
     }
 
-    Stage<T, DP, BN> ks, vs;
+    // Double buffer: while a tile is worked on, the next one is on its way, and the mask bytes of the one after that.
     uint64_t word[NW], next[NW];
-    auto fetch = [&](int tile) {
-        const int j0 = tile * BN;
-#pragma unroll
-        for (int i = 0; i < NW; ++i) next[i] = key_word(a, mask, j0 + 64 * i, n_keys);
-        // rows that no query may see are zeros: what lies there takes no part, not even as 0 * NaN
-        auto ok = [&](int r) { return (bool)(next[r >> 6 < NW ? r >> 6 : 0] >> (r & 63) & 1); };
-        ks.load(kb + (int64_t)j0 * a.k_st, a.k_st, a.D, ok);
-        vs.load(vb + (int64_t)j0 * a.v_st, a.v_st, a.D, ok);
+    bool any = false, next_any = false;                         // tiles without a visible key are passed over
+    const Stage<T, DP, BN> stage;
+    auto fetch = [&](int tile, const char *s) {
+        next_any = keys.words(next, PART);
+        if (next_any) {
+            stage.load(kb + (int64_t)tile * BN * a.k_st, a.k_st, a.D, next, s);
+            stage.load(vb + (int64_t)tile * BN * a.v_st, a.v_st, a.D, next, s + TB);
+        }
+        keys.ask((tile + 1) * BN);
     };
-    if (t < t_end) fetch(t);
-    for (int buf = 0; t < t_end; ++t, buf = (buf + 1) % NBUF) {
-        char *sk = smem + buf * 2 * TB, *sv = sk + TB;
-        if (NBUF == 1) __syncthreads();
-        ks.put(sk);
-        vs.put(sv);
+    if (NBUF == 2 && t < t_end) fetch(t, smem);
+    for (int buf = 0; t < t_end; ++t, buf ^= NBUF - 1) {
+        const char *sk = smem + buf * 2 * TB, *sv = sk + TB;
+        if (NBUF == 1) {
+            __syncthreads();                                    // everyone has read the last tile
+            fetch(t, smem);
+        }
+        tile_barrier();                                         // the tile is there (and the other buffer free)
+        any = next_any;
 #pragma unroll
         for (int i = 0; i < NW; ++i) word[i] = next[i];
-        if (t + 1 < t_end) fetch(t + 1);
-        __syncthreads();
+        if (NBUF == 2 && t + 1 < t_end) fetch(t + 1, smem + (buf ^ 1) * 2 * TB);
+        if (!any) continue;
 
         // scores of this wave's KW keys
         f32x16 s[NK];
@@ -326,7 +486,7 @@ nsd_attn_fwd_kernel(SeqArgs a)
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[n][e] = 0.0f;
 #pragma unroll
-            for (int kc = 0; kc < KC; ++kc) mma(s[n], TL::row_frag(sk, wn * KW + 32 * n + c32, kc, h), qf[kc]);
+            for (int kc = 0; kc < KC; ++kc) mma(s[n], TL::row_frag(sk, wn * KW + 32 * n, kc, lane), qf[kc]);
         }
         // the keys that this lane's row sees, of the wave's part of the tile
         const int kw0 = wn * KW;
@@ -413,44 +573,42 @@ nsd_attn_fwd_kernel(SeqArgs a)
                 o[dt][e] = x;
             }
     }
-    if (!row_ok) return;
     if (STATE || a.splits > 1) {
         const size_t at = (size_t)split * a.Z * a.Lq * (a.KVH * a.G) + row;
-        if (h == 0) {
+        if (h == 0 && row_ok) {
             a.pm[at] = m * LN2;
             a.pl[at] = l;
         }
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int d = 32 * dt + 8 * b + 4 * h;
-                if (d < a.D) store4(a.po + at * a.D + d, o[dt][4 * b], o[dt][4 * b + 1], o[dt][4 * b + 2], o[dt][4 * b + 3]);
-            }
+        put_rows<float, DP>(nullptr, o, 1.0f, a.D, lane, [&](int) { return row_ok ? a.po + at * a.D : nullptr; });
     } else {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;          // a row that sees nothing: zeros (NaN stays NaN)
-        if (h == 0 && a.lse) a.lse[((size_t)z * a.KVH + kvh) * a.R + rho] = l == 0.0f ? -__builtin_inff() : (m + __log2f(l)) * LN2;
-        T *op = static_cast<T *>(a.out) + row * a.D;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int d = 32 * dt + 8 * b + 4 * h;
-                if (d < a.D)
-                    store4(op + d, o[dt][4 * b] * inv, o[dt][4 * b + 1] * inv, o[dt][4 * b + 2] * inv, o[dt][4 * b + 3] * inv);
-            }
+        if (h == 0 && row_ok && a.lse)
+            a.lse[((size_t)z * a.KVH + kvh) * a.R + rho] = l == 0.0f ? -__builtin_inff() : (m + __log2f(l)) * LN2;
+        if (WN == 1) __syncthreads();                           // everyone is done with the tiles
+        char *mine = smem + wm * (WN > 1 ? WN * 32 * (DP + 2) * 4 : 32 * (DP * 2 + 16));    // (what only this wave has read)
+        auto place = [&](int r) {                               // of row r of the wave's 32, in elements; -1: no row
+            const int x = r0 + wm * 32 + r, i = div_g(x, a.g_magic, a.G);
+            return x < a.R ? (int64_t)((((size_t)z * a.Lq + i) * a.KVH + kvh) * a.G + (x - i * a.G)) * a.D : -1;
+        };
+        put_rows<T, DP>(mine, o, inv, a.D, lane, [&](int r) { const int64_t x = place(r); return x < 0 ? nullptr : static_cast<T *>(a.out) + x; });
+        if constexpr (sizeof(T) == 2) {
+            if (a.rest) put_rest<DP>(mine, o, inv, a.D, lane, [&](int r) { const int64_t x = place(r); return x < 0 ? nullptr : a.rest + x; });
+        }
     }
 }
 
 // ---------------------------------------------------------------------
-// the states of the splits of a row, joined: to a state (out null) or to the row itself.  One wave per row.
+// the states of the splits of a row, joined: to a state (out null) or to the row itself.  32 lanes hold a row's D
+// elements, `share` such groups (a power of two) share the splits of a row, so that a workgroup of eight groups has many
+// loads on their way where a row has many splits and works on several rows where it has few.
 // ---------------------------------------------------------------------
 struct JoinArgs {
     const float *po, *pm, *pl;
-    int splits, D, KVH, G, Lq;
+    int splits, D, KVH, G, Lq, share;
     size_t rows;
     float *so, *sm, *sl;
     void *out;
+    int8_t *rest;
     float *lse;
 };
 
@@ -458,33 +616,49 @@ template <class T>
 __global__ void __launch_bounds__(256)
 nsd_attn_join_kernel(JoinArgs a)
 {
-    const int lane = threadIdx.x & 63;
-    const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.rows) return;
-    float m = -__builtin_inff();
-    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, a.pm[s * a.rows + row]);
-    m = wave_max_f(m);
-    const float mu = m == -__builtin_inff() ? 0.0f : m;
-    float l = 0.0f;
-    for (int s = lane; s < a.splits; s += 64) l += a.pl[s * a.rows + row] * exp2_hw((a.pm[s * a.rows + row] - mu) * LOG2E);
-    l = wave_sum_f(l);
-    const float inv = a.out ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-    for (int d = 2 * lane; d < a.D; d += 128) {
-        float x = 0.0f, y = 0.0f;
-        for (int s = 0; s < a.splits; ++s) {
-            const float f = exp2_hw((a.pm[s * a.rows + row] - mu) * LOG2E);
-            const float2 p = *reinterpret_cast<const float2 *>(a.po + (s * a.rows + row) * a.D + d);
-            x = __builtin_fmaf(p.x, f, x);
-            y = __builtin_fmaf(p.y, f, y);
+    __shared__ __align__(16) float4 sum[8][32];
+    const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, part = grp % a.share;
+    const size_t row = (size_t)blockIdx.x * (8 / a.share) + grp / a.share;
+    const bool row_ok = row < a.rows;
+    float m = -__builtin_inff(), l = 0.0f, mu = 0.0f;
+    float4 x = make_float4(0, 0, 0, 0);
+    if (row_ok) {
+        for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, a.pm[s * a.rows + row]);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 32));
+        mu = m == -__builtin_inff() ? 0.0f : m;
+        for (int s = lane; s < a.splits; s += 32) l += a.pl[s * a.rows + row] * exp2_hw((a.pm[s * a.rows + row] - mu) * LOG2E);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) l += __shfl_xor(l, d, 32);
+        if (4 * lane < a.D) {
+#pragma unroll 4
+            for (int s = part; s < a.splits; s += a.share) {
+                const float f = exp2_hw((a.pm[s * a.rows + row] - mu) * LOG2E);
+                const float4 p = *reinterpret_cast<const float4 *>(a.po + (s * a.rows + row) * a.D + 4 * lane);
+                x.x = __builtin_fmaf(p.x, f, x.x);
+                x.y = __builtin_fmaf(p.y, f, x.y);
+                x.z = __builtin_fmaf(p.z, f, x.z);
+                x.w = __builtin_fmaf(p.w, f, x.w);
+            }
         }
-        x *= inv;
-        y *= inv;
+    }
+    if (a.share > 1) {
+        sum[grp][lane] = x;
+        __syncthreads();
+        for (int i = 1; i < a.share && part == 0; ++i) {
+            const float4 y = sum[grp + i][lane];
+            x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+        }
+    }
+    if (!row_ok || part) return;
+    if (4 * lane < a.D) {
         if (a.out) {
-            T *o = static_cast<T *>(a.out) + row * a.D + d;
-            o[0] = from_f<T>(x);
-            o[1] = from_f<T>(y);
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
+            store4(static_cast<T *>(a.out) + row * a.D + 4 * lane, x.x, x.y, x.z, x.w);
+            if (sizeof(T) == 2 && a.rest) *reinterpret_cast<uint32_t *>(a.rest + row * a.D + 4 * lane) = rest4(x.x, x.y, x.z, x.w);
         } else {
-            *reinterpret_cast<float2 *>(a.so + row * a.D + d) = make_float2(x, y);
+            store4(a.so + row * a.D + 4 * lane, x.x, x.y, x.z, x.w);
         }
     }
     if (lane == 0) {
@@ -501,26 +675,44 @@ nsd_attn_join_kernel(JoinArgs a)
     }
 }
 
+// sums of the splits of a gradient, rounded to the element type (n a multiple of 4)
+template <class T>
+__global__ void __launch_bounds__(256)
+nsd_attn_sum_kernel(const float *part, size_t n, int splits, T *out)
+{
+    const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    float4 x = *reinterpret_cast<const float4 *>(part + i);
+#pragma unroll 4
+    for (int s = 1; s < splits; ++s) {
+        const float4 y = *reinterpret_cast<const float4 *>(part + s * n + i);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    }
+    store4(out + i, x.x, x.y, x.z, x.w);
+}
+
 // ---------------------------------------------------------------------
 // backward, first part: dQ = scale dS K with dS = P (dP - delta), dP = dO V^T, delta = rowsum(dO O), which it leaves for
 // the second part.  Layout of the forward: a wave owns 32 rows, S^T and dP^T are computed from the same tiles.
 // ---------------------------------------------------------------------
-template <class T, int DP, int BN>
-__global__ void __launch_bounds__(256)
+template <class T, int DP, int WM, int NK, int NBUF>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1)
 nsd_attn_bwd_q_kernel(SeqArgs a)
 {
-    constexpr int BM = 128, NK = BN / 32, DT = DP / 32, KC = DP / 16;
+    constexpr int WN = 4 / WM, BM = 32 * WM, BN = 32 * NK * WN, DT = DP / 32, KC = DP / 16;
+    constexpr int NW = BN > 64 ? BN / 64 : 1;
     using TL = Tile<T, DP>;
     constexpr int TB = BN * TL::RB;
-    __shared__ __align__(16) char smem[4 * TB];
+    static_assert(WN == 1 || 2 * NBUF * TB >= 4 * 32 * DP * 4, "the waves' sums meet in the tiles' place");
+    __shared__ __align__(16) char smem[2 * NBUF * TB];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c32 = lane & 31;
+    const int wm = w % WM, wn = w / WM;
     const int rtiles = (a.R + BM - 1) / BM;
-    int bid = blockIdx.x;
-    const int rt = rtiles - 1 - bid % rtiles;
-    bid /= rtiles;
-    const int kvh = bid % a.KVH, z = bid / a.KVH;
+    int pair, tile;
+    work_of(blockIdx.x, rtiles, a.Z * a.KVH * a.splits, a.batch, pair, tile);
+    const int rt = rtiles - 1 - tile, split = pair % a.splits, kvh = pair / a.splits % a.KVH, z = pair / a.splits / a.KVH;
     const uint8_t *mask = a.mask ? a.mask + (size_t)z * a.Lk : nullptr;
-    const int r0 = rt * BM, rho = r0 + w * 32 + c32;
+    const int r0 = rt * BM, rho = r0 + wm * 32 + c32;
     const bool row_ok = rho < a.R;
     const int off = a.Lk - a.Lq;
     const int i_row = div_g(row_ok ? rho : a.R - 1, a.g_magic, a.G);
@@ -528,12 +720,16 @@ nsd_attn_bwd_q_kernel(SeqArgs a)
     const int last = a.causal ? i_row + off : a.Lk;
     int kend = a.Lk;
     if (a.causal) kend = min(kend, div_g(min(r0 + BM, a.R) - 1, a.g_magic, a.G) + off + 1);
-    const int t_end = kend > 0 ? (kend + BN - 1) / BN : 0;
+    const int t_end = min((split + 1) * a.split_tiles, kend > 0 ? (kend + BN - 1) / BN : 0);
+    int t = split * a.split_tiles;
     const T *kb = static_cast<const T *>(a.k) + z * a.k_sz + kvh * a.k_sh;
     const T *vb = static_cast<const T *>(a.v) + z * a.v_sz + kvh * a.v_sh;
     const size_t row = ((size_t)z * a.Lq + i_row) * (a.KVH * a.G) + head;
     const size_t prow = ((size_t)z * a.KVH + kvh) * a.R + rho;
 
+    constexpr uint64_t PART = BN < 64 ? (1ull << (BN & 63)) - 1 : ~0ull;
+    KeyMask<NW> keys{mask, a.Lk, {}};
+    if (t < t_end) keys.ask(t * BN);
     Frag<T> qf[KC], gf[KC];
     float delta = 0.0f;
     {
@@ -543,11 +739,13 @@ nsd_attn_bwd_q_kernel(SeqArgs a)
         for (int kc = 0; kc < KC; ++kc) {
             qf[kc] = mem_frag(qp, 16 * kc + 8 * h, a.D, row_ok);
             gf[kc] = mem_frag(gp, 16 * kc + 8 * h, a.D, row_ok);
-            delta = frag_dot(gf[kc], mem_frag(op, 16 * kc + 8 * h, a.D, row_ok), delta);
+            const Frag<T> of = mem_frag(op, 16 * kc + 8 * h, a.D, row_ok);
+            delta = frag_dot(gf[kc], of, delta);
+            if (a.rest && row_ok && 16 * kc + 8 * h < a.D) delta = rest_dot(gf[kc], of, a.rest + row * a.D + 16 * kc + 8 * h, delta);
         }
         delta = half_sum(delta);
     }
-    if (h == 0 && row_ok) a.delta[prow] = delta;
+    if (h == 0 && row_ok && wn == 0 && split == 0) a.delta[prow] = delta;
     const float lse2 = row_ok ? a.lse[prow] * LOG2E : 0.0f;
     f32x16 o[DT];
 #pragma unroll
@@ -555,34 +753,43 @@ nsd_attn_bwd_q_kernel(SeqArgs a)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
 
-    Stage<T, DP, BN> ks, vs;
-    uint64_t word = 0, next = 0;
-    auto fetch = [&](int tile) {
-        const int j0 = tile * BN;
-        next = key_word(a, mask, j0, a.Lk);
-        auto ok = [&](int r) { return (bool)(next >> (r & 63) & 1); };
-        ks.load(kb + (int64_t)j0 * a.k_st, a.k_st, a.D, ok);
-        vs.load(vb + (int64_t)j0 * a.v_st, a.v_st, a.D, ok);
+    // Double buffer: while a tile is worked on, the next one is on its way, and the mask bytes of the one after that.
+    uint64_t word[NW], next[NW];
+    bool any = false, next_any = false;                         // tiles without a visible key are passed over
+    const Stage<T, DP, BN> stage;
+    auto fetch = [&](int tile, const char *s) {
+        next_any = keys.words(next, PART);
+        if (next_any) {
+            stage.load(kb + (int64_t)tile * BN * a.k_st, a.k_st, a.D, next, s);
+            stage.load(vb + (int64_t)tile * BN * a.v_st, a.v_st, a.D, next, s + TB);
+        }
+        keys.ask((tile + 1) * BN);
     };
-    if (t_end > 0) fetch(0);
-    for (int t = 0, buf = 0; t < t_end; ++t, buf ^= 1) {
-        char *sk = smem + buf * 2 * TB, *sv = sk + TB;
-        ks.put(sk);
-        vs.put(sv);
-        word = next;
-        if (t + 1 < t_end) fetch(t + 1);
-        __syncthreads();
-        const int n_vis = last + 1 - t * BN;
-        const uint64_t vis = n_vis <= 0 ? 0 : n_vis < 64 ? word & ((1ull << n_vis) - 1) : word;
+    if (NBUF == 2 && t < t_end) fetch(t, smem);
+    for (int buf = 0; t < t_end; ++t, buf ^= NBUF - 1) {
+        const char *sk = smem + buf * 2 * TB, *sv = sk + TB;
+        if (NBUF == 1) {
+            __syncthreads();                                    // everyone has read the last tile
+            fetch(t, smem);
+        }
+        tile_barrier();                                         // the tile is there (and the other buffer free)
+        any = next_any;
 #pragma unroll
+        for (int i = 0; i < NW; ++i) word[i] = next[i];
+        if (NBUF == 2 && t + 1 < t_end) fetch(t + 1, smem + (buf ^ 1) * 2 * TB);
+        if (!any) continue;
+        const int kw0 = wn * 32 * NK, n_vis = last + 1 - (t * BN + kw0);
+        uint64_t vis = word[NW > 1 ? kw0 >> 6 : 0] >> (kw0 & 63);
+        vis = n_vis <= 0 ? 0 : n_vis < 64 ? vis & ((1ull << n_vis) - 1) : vis;
+#pragma unroll 1
         for (int n = 0; n < NK; ++n) {
             f32x16 s, dp;
 #pragma unroll
             for (int e = 0; e < 16; ++e) { s[e] = 0.0f; dp[e] = -delta; }
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) {
-                mma(s, TL::row_frag(sk, 32 * n + c32, kc, h), qf[kc]);
-                mma(dp, TL::row_frag(sv, 32 * n + c32, kc, h), gf[kc]);
+                mma(s, TL::row_frag(sk, kw0 + 32 * n, kc, lane), qf[kc]);
+                mma(dp, TL::row_frag(sv, kw0 + 32 * n, kc, lane), gf[kc]);
             }
             const uint32_t bits = (uint32_t)(vis >> (32 * n)) >> (4 * h);
 #pragma unroll
@@ -594,45 +801,64 @@ nsd_attn_bwd_q_kernel(SeqArgs a)
             for (int c = 0; c < 2; ++c) {
                 const Frag<T> p = acc_frag(s, c, T{});
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) mma(o[dt], TL::col_frag(sk, 32 * n + 16 * c, dt, lane), p);
+                for (int dt = 0; dt < DT; ++dt) mma(o[dt], TL::col_frag(sk, kw0 + 32 * n + 16 * c, dt, lane), p);
             }
         }
     }
-    if (!row_ok) return;
-    T *op = static_cast<T *>(a.dq) + row * a.D;
+    if constexpr (WN > 1) {                                     // the sums of a row's waves meet
+        float *js = reinterpret_cast<float *>(smem);
+        __syncthreads();
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int d = 32 * dt + 8 * b + 4 * h;
-            if (d < a.D)
-                store4(op + d, o[dt][4 * b] * a.scale, o[dt][4 * b + 1] * a.scale, o[dt][4 * b + 2] * a.scale,
-                       o[dt][4 * b + 3] * a.scale);
-        }
+            for (int e = 0; e < 16; ++e)
+                js[(w * DP + 32 * dt + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + c32] = o[dt][e];
+        __syncthreads();
+        if (wn) return;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+#pragma unroll
+                for (int i = 1; i < WN; ++i)
+                    o[dt][e] += js[((wm + i * WM) * DP + 32 * dt + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + c32];
+    }
+    if (a.splits > 1) {
+        float *pp = row_ok ? a.part + ((size_t)split * a.Z * a.Lq * (a.KVH * a.G) + row) * a.D : nullptr;
+        put_rows<float, DP>(nullptr, o, a.scale, a.D, lane, [&](int) { return pp; });
+        return;
+    }
+    if (WN == 1) __syncthreads();                               // everyone is done with the tiles
+    put_rows<T, DP>(smem + wm * (WN > 1 ? 32 * DP * 4 : 32 * (DP * 2 + 16)), o, a.scale, a.D, lane, [&](int r) {
+        const int x = r0 + wm * 32 + r, i = div_g(x, a.g_magic, a.G);
+        return x < a.R ? static_cast<T *>(a.dq) + ((((size_t)z * a.Lq + i) * a.KVH + kvh) * a.G + (x - i * a.G)) * a.D : nullptr;
+    });
 }
 
 // ---------------------------------------------------------------------
 // backward, second part: dV = P^T dO, dK = scale dS^T Q.  A wave owns 32 keys, whose K and V stay in its registers, and
-// the workgroup's four walk over the rows of all G heads (their gradients of a shared head add up in the accumulators):
-// S = Q K^T and dP = dO V^T with a lane per key, so that P and dS lie as the B operands of dV^T = dO^T P and
-// dK^T = Q^T dS.
+// walks over the rows of all G heads (their gradients of a shared head add up in the accumulators): S = Q K^T and
+// dP = dO V^T with a lane per key, so that P and dS lie as the B operands of dV^T = dO^T P and dK^T = Q^T dS.  Of a
+// workgroup's waves WK lie along the keys and WR = 4 / WK share the rows of a tile, NS sub-tiles of 32 each; their sums
+// meet at the end.  Rows are walked from the last one, which all keys see: the workgroups of a kv head then read the same
+// rows at the same time.
 // ---------------------------------------------------------------------
-template <class T, int DP, int BM>
-__global__ void __launch_bounds__(256)
+template <class T, int DP, int WK, int NS, int NBUF>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1)
 nsd_attn_bwd_kv_kernel(SeqArgs a)
 {
-    constexpr int BN = 128, NM = BM / 32, DT = DP / 32, KC = DP / 16;
+    constexpr int WR = 4 / WK, BN = 32 * WK, BM = 32 * WR * NS, DT = DP / 32, KC = DP / 16;
     using TL = Tile<T, DP>;
     constexpr int TB = BM * TL::RB;
-    __shared__ __align__(16) char smem[4 * TB];
-    __shared__ __align__(16) float stat[2][2][BM];
+    static_assert(WR == 1 || 2 * NBUF * TB >= 4 * 32 * DP * 4, "the waves' sums meet in the tiles' place");
+    __shared__ __align__(16) char smem[2 * NBUF * TB];
+    __shared__ __align__(16) float stat[NBUF][2][BM];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c32 = lane & 31;
-    const int ktiles = (a.Lk + BN - 1) / BN;
-    int bid = blockIdx.x;
-    const int kt = bid % ktiles;                                // the first keys are seen by most rows
-    bid /= ktiles;
-    const int kvh = bid % a.KVH, z = bid / a.KVH;
-    const int j = kt * BN + w * 32 + c32;
+    const int wk = w % WK, wr = w / WK;
+    int pair, kt;                                               // the first keys are seen by most rows
+    work_of(blockIdx.x, (a.Lk + BN - 1) / BN, a.Z * a.KVH * a.splits, a.batch, pair, kt);
+    const int split = pair % a.splits, kvh = pair / a.splits % a.KVH, z = pair / a.splits / a.KVH;
+    const int j = kt * BN + wk * 32 + c32;
     bool key_ok = j < a.Lk;
     if (key_ok && a.mask) key_ok = a.mask[(size_t)z * a.Lk + j] != 0;
     const int off = a.Lk - a.Lq;
@@ -648,8 +874,14 @@ nsd_attn_bwd_kv_kernel(SeqArgs a)
     const int64_t lo = a.causal ? (int64_t)(j - off) * a.G : 0;
     const int first = !key_ok ? 0x7fffffff : lo > 0 ? (int)min(lo, (int64_t)a.R) : 0;
     const int64_t lo0 = a.causal ? (int64_t)(kt * BN - off) * a.G : 0;
-    const int t_end = (a.R + BM - 1) / BM;
-    int t = lo0 > 0 ? (int)min(lo0 / BM, (int64_t)t_end) : 0;
+    const int t_last = (a.R + BM - 1) / BM - 1;
+    int t_first = lo0 > 0 ? (int)min(lo0 / BM, (int64_t)t_last + 1) : 0, t = t_last;
+    if (a.splits > 1) {                                         // this split's part of the rows that see these keys
+        const int n = (t_last + 1 - t_first + a.splits - 1) / a.splits;
+        t -= split * n;
+        t_first = max(t_first, t - n + 1);
+    }
+    if (a.mask && !__syncthreads_or(key_ok)) t_first = t + 1;   // keys that nobody sees
 
     f32x16 dk[DT], dv[DT];
 #pragma unroll
@@ -657,21 +889,20 @@ nsd_attn_bwd_kv_kernel(SeqArgs a)
 #pragma unroll
         for (int e = 0; e < 16; ++e) { dk[dt][e] = 0.0f; dv[dt][e] = 0.0f; }
 
-    constexpr int PR = TL::PR, U = BM * PR / 256, EP = 16 / (int)sizeof(T);
-    uint4 qx[U], gx[U];
     float st_l = 0.0f, st_d = 0.0f;
     const size_t pbase = ((size_t)z * a.KVH + kvh) * a.R;
-    auto fetch = [&](int tile) {
+    const T *qb = static_cast<const T *>(a.q) + z * a.q_sz, *gb = static_cast<const T *>(a.dout) + (size_t)z * a.Lq * (a.KVH * a.G) * a.D;
+    const Stage<T, DP, BM> stage;
+    auto fetch = [&](int tile, const char *sm) {
+        const uint32_t dst = lds_at(sm);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = (int)threadIdx.x + 256 * u, r = tile * BM + i / PR, p = i % PR;
-            qx[u] = gx[u] = make_uint4(0, 0, 0, 0);
-            if (r < a.R && p * EP < a.D) {
-                const int tok = div_g(r, a.g_magic, a.G), hd = kvh * a.G + r - tok * a.G;
-                qx[u] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + z * a.q_sz + tok * a.q_st + hd * a.q_sh + p * EP);
-                gx[u] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.dout) +
-                                                         (((size_t)z * a.Lq + tok) * (a.KVH * a.G) + hd) * a.D + p * EP);
-            }
+        for (int u = 0; u < stage.U; ++u) {
+            const int r = tile * BM + stage.chunk_row(u) + stage.row, e = stage.chunk_elem(u) + stage.elem;
+            const bool ok = r < a.R && e < a.D;
+            const int tok = div_g(r, a.g_magic, a.G), hd = kvh * a.G + r - tok * a.G;
+            const uint64_t zero = (uint64_t)zero_page;
+            to_lds(ok ? (uint64_t)(qb + tok * a.q_st + hd * a.q_sh + e) : zero, stage.place(dst, u));
+            to_lds(ok ? (uint64_t)(gb + ((size_t)tok * (a.KVH * a.G) + hd) * a.D + e) : zero, stage.place(dst + TB, u));
         }
         if (threadIdx.x < BM) {
             const int r = tile * BM + (int)threadIdx.x;
@@ -679,37 +910,34 @@ nsd_attn_bwd_kv_kernel(SeqArgs a)
             st_d = r < a.R ? a.delta[pbase + r] : 0.0f;
         }
     };
-    if (t < t_end) fetch(t);
-    for (int buf = 0; t < t_end; ++t, buf ^= 1) {
-        char *sq = smem + buf * 2 * TB, *sg = sq + TB;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = (int)threadIdx.x + 256 * u;
-            *reinterpret_cast<uint4 *>(sq + TL::at(i / PR, i % PR)) = qx[u];
-            *reinterpret_cast<uint4 *>(sg + TL::at(i / PR, i % PR)) = gx[u];
-        }
+    auto put_stat = [&](int b) {
         if (threadIdx.x < BM) {
-            stat[buf][0][threadIdx.x] = st_l;
-            stat[buf][1][threadIdx.x] = st_d;
+            stat[b][0][threadIdx.x] = st_l;
+            stat[b][1][threadIdx.x] = st_d;
         }
-        if (t + 1 < t_end) fetch(t + 1);
-        __syncthreads();
-#pragma unroll
-        for (int n = 0; n < NM; ++n) {
+    };
+    if (NBUF == 2 && t >= t_first) {
+        fetch(t, smem);
+        put_stat(0);
+    }
+    for (int buf = 0; t >= t_first; --t, buf ^= NBUF - 1) {
+        char *sq = smem + buf * 2 * TB, *sg = sq + TB;
+        if (NBUF == 1) {
+            __syncthreads();                                    // everyone has read the last tile
+            fetch(t, smem);
+            put_stat(0);
+        }
+        tile_barrier();
+        if (NBUF == 2 && t > t_first) fetch(t - 1, smem + (buf ^ 1) * 2 * TB);
+#pragma unroll 1
+        for (int i = 0; i < NS; ++i) {
+            const int n = wr + WR * i;
+            const int thr = first - (t * BM + 32 * n + 4 * h);
             f32x16 s, dp;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const float4 x = *reinterpret_cast<const float4 *>(&stat[buf][1][32 * n + 8 * b + 4 * h]);
-                dp[4 * b] = -x.x; dp[4 * b + 1] = -x.y; dp[4 * b + 2] = -x.z; dp[4 * b + 3] = -x.w;
-            }
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
-            for (int kc = 0; kc < KC; ++kc) {
-                mma(s, TL::row_frag(sq, 32 * n + c32, kc, h), kf[kc]);
-                mma(dp, TL::row_frag(sg, 32 * n + c32, kc, h), vf[kc]);
-            }
-            const int thr = first - (t * BM + 32 * n + 4 * h);
+            for (int kc = 0; kc < KC; ++kc) mma(s, TL::row_frag(sq, 32 * n, kc, lane), kf[kc]);
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 const float4 x = *reinterpret_cast<const float4 *>(&stat[buf][0][32 * n + 8 * b + 4 * h]);
@@ -718,38 +946,77 @@ nsd_attn_bwd_kv_kernel(SeqArgs a)
                 for (int e = 0; e < 4; ++e) {
                     const float p = exp2_hw(__builtin_fmaf(s[4 * b + e], a.scale2, -ls[e]));
                     s[4 * b + e] = 8 * b + e >= thr ? p : 0.0f;
-                    dp[4 * b + e] = 8 * b + e >= thr ? p * dp[4 * b + e] : 0.0f;
                 }
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const Frag<T> p = acc_frag(s, c, T{}), ds = acc_frag(dp, c, T{});
+                const Frag<T> p = acc_frag(s, c, T{});
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    mma(dv[dt], TL::col_frag(sg, 32 * n + 16 * c, dt, lane), p);
-                    mma(dk[dt], TL::col_frag(sq, 32 * n + 16 * c, dt, lane), ds);
-                }
+                for (int dt = 0; dt < DT; ++dt) mma(dv[dt], TL::col_frag(sg, 32 * n + 16 * c, dt, lane), p);
+            }
+
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const float4 x = *reinterpret_cast<const float4 *>(&stat[buf][1][32 * n + 8 * b + 4 * h]);
+                dp[4 * b] = -x.x; dp[4 * b + 1] = -x.y; dp[4 * b + 2] = -x.z; dp[4 * b + 3] = -x.w;
+            }
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) mma(dp, TL::row_frag(sg, 32 * n, kc, lane), vf[kc]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dp[e] = s[e] != 0.0f ? s[e] * dp[e] : 0.0f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const Frag<T> ds = acc_frag(dp, c, T{});
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) mma(dk[dt], TL::col_frag(sq, 32 * n + 16 * c, dt, lane), ds);
             }
         }
+        if (NBUF == 2 && t > t_first) put_stat(buf ^ 1);
     }
-    if (j >= a.Lk) return;
-    const size_t at = (((size_t)z * a.Lk + j) * a.KVH + kvh) * a.D;
-    T *pk = static_cast<T *>(a.dk) + at, *pv = static_cast<T *>(a.dv) + at;
+    if constexpr (WR > 1) {
+        float *js = reinterpret_cast<float *>(smem);
+        f32x16 *acc[2] = {dk, dv};
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+        for (int x = 0; x < 2; ++x) {
+            __syncthreads();
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int d = 32 * dt + 8 * b + 4 * h;
-            if (d >= a.D) continue;
-            float x[4], y[4];
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {                       // a masked key has no part in anything
-                x[e] = key_ok ? dk[dt][4 * b + e] * a.scale : 0.0f;
-                y[e] = key_ok ? dv[dt][4 * b + e] : 0.0f;
+                for (int e = 0; e < 16; ++e)
+                    js[(w * DP + 32 * dt + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + c32] = acc[x][dt][e];
+            __syncthreads();
+            if (wr == 0) {
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+#pragma unroll
+                        for (int i = 1; i < WR; ++i)
+                            acc[x][dt][e] += js[((wk + i * WK) * DP + 32 * dt + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + c32];
             }
-            store4(pk + d, x[0], x[1], x[2], x[3]);
-            store4(pv + d, y[0], y[1], y[2], y[3]);
         }
+        if (wr) return;
+    }
+    if (!key_ok) {                                              // a masked key has no part in anything
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) { dk[dt][e] = 0.0f; dv[dt][e] = 0.0f; }
+    }
+    const size_t all = (size_t)a.Z * a.Lk * a.KVH * a.D;
+    auto place = [&](int r) {                                   // of key r of the wave's 32, in elements; -1: no key
+        const int x = kt * BN + wk * 32 + r;
+        return x < a.Lk ? (int64_t)((((size_t)z * a.Lk + x) * a.KVH + kvh) * a.D) : -1;
+    };
+    if (a.splits > 1) {
+        const int64_t x = place(c32);
+        put_rows<float, DP>(nullptr, dk, a.scale, a.D, lane, [&](int) { return x < 0 ? nullptr : a.part + split * all + x; });
+        put_rows<float, DP>(nullptr, dv, 1.0f, a.D, lane, [&](int) { return x < 0 ? nullptr : a.part_v + split * all + x; });
+        return;
+    }
+    char *mine = smem + wk * 32 * DP * 4;                       // (what only this wave has read)
+    put_rows<T, DP>(mine, dk, a.scale, a.D, lane, [&](int r) { const int64_t x = place(r); return x < 0 ? nullptr : static_cast<T *>(a.dk) + x; });
+    put_rows<T, DP>(mine, dv, 1.0f, a.D, lane, [&](int r) { const int64_t x = place(r); return x < 0 ? nullptr : static_cast<T *>(a.dv) + x; });
 }
 
 // ---------------------------------------------------------------------
@@ -757,53 +1024,97 @@ nsd_attn_bwd_kv_kernel(SeqArgs a)
 // ---------------------------------------------------------------------
 constexpr int CUS = 256;
 
-struct FwdPlan { int wm, bn, rtiles, splits, split_tiles; };
+struct Plan { int wave_rows, bn, tiles, splits, split_tiles; };
 
 int dp_of(int D) { return D <= 64 ? 64 : 128; }
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Row tiles of 128 (four waves along the rows) unless there are at most 64 or 32 rows: the waves then share the keys of
-// a tile.  The keys are split over several workgroups while there are fewer workgroups than CUs.
-FwdPlan fwd_plan(int Z, int KVH, int R, int Lk, int D, int dtype)
+// How often the walk over `steps` tiles is split so that `room` workgroups are on the card: whole shares, as a few more
+// workgroups than there is room for cost a second round; no share shorter than `least`, below which the join costs more
+// than the split gives.
+void split_walk(Plan &p, int64_t wgs, int64_t steps, int64_t room, int64_t least)
 {
-    FwdPlan p;
-    p.wm = R <= 32 ? 1 : R <= 64 ? 2 : 4;
-    const int kw = dtype == 0 ? 32 : p.wm == 1 ? 32 : 64;
-    p.bn = kw * (4 / p.wm);
-    p.rtiles = (R + 32 * p.wm - 1) / (32 * p.wm);
-    const int64_t wgs = (int64_t)p.rtiles * KVH * Z;
-    const int tiles = (Lk + p.bn - 1) / p.bn;
-    p.splits = 1;
-    if (wgs < CUS && tiles > 1) {
-        int64_t s = (2 * CUS + wgs - 1) / wgs;
-        s = s < tiles ? s : tiles;
-        p.split_tiles = (int)((tiles + s - 1) / s);
-        p.splits = (tiles + p.split_tiles - 1) / p.split_tiles;
-    } else {
-        p.split_tiles = tiles > 0 ? tiles : 1;
-    }
+    int64_t s = wgs > 0 ? room / wgs : 1;
+    s = s > steps / least ? steps / least : s;
+    p.split_tiles = (int)(s > 1 ? div_up(steps, s) : steps > 0 ? steps : 1);
+    p.splits = (int)(s > 1 ? div_up(steps, p.split_tiles) : 1);
+}
+
+// Forward: row tiles of 128 (four waves along the rows) unless there are at most 64 or 32 rows: the waves then share the
+// keys of a tile.
+Plan fwd_plan(int Z, int KVH, int R, int Lk, int D, int dtype)
+{
+    Plan p;
+    p.wave_rows = R <= 32 ? 1 : R <= 64 ? 2 : 4;
+    p.bn = (dtype == 0 || p.wave_rows == 1 ? 32 : 64) * (4 / p.wave_rows);
+    p.tiles = (int)div_up(R, 32 * p.wave_rows);
+    split_walk(p, (int64_t)p.tiles * KVH * Z, div_up(Lk, p.bn), 2 * CUS, dtype == 0 ? 1 : 4);
     return p;
 }
 
+// Backward, dQ: 128 rows where that makes a workgroup for every CU, else 64 or 32 (the waves share the keys).
+Plan bwd_q_plan(int Z, int KVH, int R, int Lk, int D, int dtype)
+{
+    Plan p;
+    const int64_t pairs = (int64_t)Z * KVH;
+    p.wave_rows = pairs * div_up(R, 128) >= CUS ? 4 : pairs * div_up(R, 64) >= CUS ? 2 : 1;
+    p.bn = p.wave_rows == 4 ? (dtype == 0 && dp_of(D) == 128 ? 32 : 64) : 32 * (4 / p.wave_rows);
+    p.tiles = (int)div_up(R, 32 * p.wave_rows);
+    split_walk(p, p.tiles * pairs, div_up(Lk, p.bn), CUS, dtype == 0 ? 1 : 8);
+    return p;
+}
+
+// Backward, dK and dV: 64 keys (two waves along the keys, two along the rows), or 32 where that leaves CUs without work.
+// Four waves along the keys, 128 of them, are slower: 119 against 86 us at 8 x 640 positions, 1439 against 1014 us at one
+// sequence of 8192 (24 query heads, 8 kv heads of 128): half as many workgroups, and unequal ones under a causal mask.
+Plan bwd_kv_plan(int Z, int KVH, int R, int Lk, int D, int dtype)
+{
+    Plan p;
+    const int64_t pairs = (int64_t)Z * KVH;
+    p.wave_rows = pairs * div_up(Lk, 64) >= CUS / 2 ? 2 : 1;       // (waves along the keys here)
+    p.bn = 32 * p.wave_rows;
+    p.tiles = (int)div_up(Lk, p.bn);
+    split_walk(p, p.tiles * pairs, div_up(R, 32 * (4 / p.wave_rows)), CUS, dtype == 0 ? 1 : 8);
+    return p;
+}
+
+// pairs of an XCD that are worked on together: two rounds of its 64 workgroups
+int pair_batch(int64_t pairs, int64_t tiles)
+{
+    const int64_t per = pairs % 8 == 0 ? pairs / 8 : pairs, b = pairs % 8 == 0 ? 128 / tiles : per;
+    return (int)(b < 1 ? 1 : b > per ? per : b);
+}
+
+dim3 grid_of(SeqArgs &a, const Plan &p)
+{
+    const int64_t pairs = (int64_t)a.KVH * a.Z * p.splits;
+    a.splits = p.splits;
+    a.split_tiles = p.split_tiles;
+    a.batch = pair_batch(pairs, p.tiles);
+    return dim3((unsigned)(p.tiles * pairs));
+}
+
 template <class T, int DP, bool STATE>
-void launch_fwd(const SeqArgs &a, const FwdPlan &p, hipStream_t s)
+void launch_fwd(SeqArgs a, const Plan &p, hipStream_t s)
 {
     constexpr bool F = sizeof(T) == 4;
-    const dim3 grid((unsigned)((int64_t)p.rtiles * a.KVH * a.Z * p.splits)), block(256);
-    if (p.wm == 4) hipLaunchKernelGGL((nsd_attn_fwd_kernel<T, DP, 4, F ? 32 : 64, 2, STATE>), grid, block, 0, s, a);
-    else if (p.wm == 2) hipLaunchKernelGGL((nsd_attn_fwd_kernel<T, DP, 2, F ? 32 : 64, F && DP == 128 ? 2 : 1, STATE>), grid, block, 0, s, a);
+    const dim3 grid = grid_of(a, p), block(256);
+    if (p.wave_rows == 4) hipLaunchKernelGGL((nsd_attn_fwd_kernel<T, DP, 4, F ? 32 : 64, 2, STATE>), grid, block, 0, s, a);
+    else if (p.wave_rows == 2) hipLaunchKernelGGL((nsd_attn_fwd_kernel<T, DP, 2, F ? 32 : 64, F && DP == 128 ? 2 : 1, STATE>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((nsd_attn_fwd_kernel<T, DP, 1, 32, F && DP == 128 ? 1 : 2, STATE>), grid, block, 0, s, a);
 }
 
-int run_join(const JoinArgs &j, int dtype, hipStream_t s)
+int run_join(JoinArgs j, int dtype, hipStream_t s)
 {
-    const dim3 grid((unsigned)((j.rows + 3) / 4)), block(256);
+    j.share = j.splits >= 8 ? 8 : j.splits >= 4 ? 4 : 2;
+    const dim3 grid((unsigned)((j.rows * j.share + 7) / 8)), block(256);
     if (dtype == 0) hipLaunchKernelGGL(nsd_attn_join_kernel<float>, grid, block, 0, s, j);
     else hipLaunchKernelGGL(nsd_attn_join_kernel<BF16>, grid, block, 0, s, j);
     return (int)hipGetLastError();
 }
 
 template <bool STATE>
-int run_fwd(const SeqArgs &a, const FwdPlan &p, int dtype, hipStream_t s)
+int run_fwd(const SeqArgs &a, const Plan &p, int dtype, hipStream_t s)
 {
     if (dtype == 0) {
         if (dp_of(a.D) == 64) launch_fwd<float, 64, STATE>(a, p, s);
@@ -815,15 +1126,42 @@ int run_fwd(const SeqArgs &a, const FwdPlan &p, int dtype, hipStream_t s)
     return (int)hipGetLastError();
 }
 
-template <class T, int DP>
-void launch_bwd(const SeqArgs &a, hipStream_t s)
+template <class T>
+void launch_sum(const float *part, size_t n, int splits, void *out, hipStream_t s)
 {
-    constexpr int BN = sizeof(T) == 4 && DP == 128 ? 32 : 64;
+    hipLaunchKernelGGL(nsd_attn_sum_kernel<T>, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s, part, n, splits, (T *)out);
+}
+
+// Scratch of the backward pass: the rows' delta, then the parts of dQ, and in the same place those of dK and dV.
+struct BwdScratch { size_t delta, q, kv; };
+BwdScratch bwd_scratch(const Plan &q, const Plan &kv, size_t rows, size_t keys, size_t D)
+{
+    return {(rows + 3) / 4 * 16, q.splits > 1 ? q.splits * rows * D * 4 : 0, kv.splits > 1 ? 2 * kv.splits * keys * D * 4 : 0};
+}
+
+template <class T, int DP>
+void launch_bwd(SeqArgs a, const Plan &q, const Plan &kv, hipStream_t s)
+{
+    constexpr bool F = sizeof(T) == 4, F128 = F && DP == 128;
     const dim3 block(256);
-    if (a.R > 0)
-        hipLaunchKernelGGL((nsd_attn_bwd_q_kernel<T, DP, BN>), dim3((unsigned)((int64_t)((a.R + 127) / 128) * a.KVH * a.Z)), block, 0, s, a);
-    if (a.Lk > 0)
-        hipLaunchKernelGGL((nsd_attn_bwd_kv_kernel<T, DP, 32>), dim3((unsigned)((int64_t)((a.Lk + 127) / 128) * a.KVH * a.Z)), block, 0, s, a);
+    const size_t nq = (size_t)a.Z * a.Lq * a.KVH * a.G * a.D, nk = (size_t)a.Z * a.Lk * a.KVH * a.D;
+    if (a.R > 0) {
+        const dim3 grid = grid_of(a, q);
+        if (q.wave_rows == 4) hipLaunchKernelGGL((nsd_attn_bwd_q_kernel<T, DP, 4, F128 ? 1 : 2, 2>), grid, block, 0, s, a);
+        else if (q.wave_rows == 2) hipLaunchKernelGGL((nsd_attn_bwd_q_kernel<T, DP, 2, 1, 2>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((nsd_attn_bwd_q_kernel<T, DP, 1, 1, F128 ? 1 : 2>), grid, block, 0, s, a);
+        if (q.splits > 1) launch_sum<T>(a.part, nq, q.splits, a.dq, s);
+    }
+    if (a.Lk > 0) {
+        const dim3 grid = grid_of(a, kv);
+        a.part_v = a.part + kv.splits * nk;
+        if (kv.wave_rows == 2) hipLaunchKernelGGL((nsd_attn_bwd_kv_kernel<T, DP, 2, 1, 2>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((nsd_attn_bwd_kv_kernel<T, DP, 1, 1, F128 ? 1 : 2>), grid, block, 0, s, a);
+        if (kv.splits > 1) {
+            launch_sum<T>(a.part, nk, kv.splits, a.dk, s);
+            launch_sum<T>(a.part_v, nk, kv.splits, a.dv, s);
+        }
+    }
 }
 
 bool al16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
@@ -870,23 +1208,22 @@ extern "C" int64_t nsd_attn_fwd_workspace(const NsdSeqAttn *p)
 {
     if (!p || p->kv_heads < 1 || p->heads < 1 || p->hd < 1 || p->batch < 1 || p->len_q < 1) return 0;
     const int G = p->heads / p->kv_heads;
-    const FwdPlan f = fwd_plan(p->batch, p->kv_heads, p->len_q * G, p->len_k, p->hd, p->dtype);
+    const Plan f = fwd_plan(p->batch, p->kv_heads, p->len_q * G, p->len_k, p->hd, p->dtype);
     return f.splits > 1 ? (int64_t)f.splits * p->batch * p->len_q * p->heads * (p->hd + 2) * 4 : 0;
 }
 
-extern "C" int nsd_attn_fwd(const void *q, const void *k, const void *v, const NsdSeqAttn *p, void *out, float *lse,
+extern "C" int nsd_attn_fwd(const void *q, const void *k, const void *v, const NsdSeqAttn *p, void *out, float *lse, int8_t *rest,
                             void *ws, int64_t ws_bytes, void *stream)
 {
     SeqArgs a;
     if (const int rc = seq_args(p, q, k, v, a)) return rc;
     if (p->batch == 0 || p->len_q == 0) return NSD_OK;
     if (!out) return NSD_E_NULL;
-    if (!al16(out) || !al16(ws)) return NSD_E_ALIGN;
-    const FwdPlan f = fwd_plan(a.Z, a.KVH, a.R, a.Lk, a.D, p->dtype);
-    a.splits = f.splits;
-    a.split_tiles = f.split_tiles;
+    if (!al16(out) || !al16(rest) || !al16(ws)) return NSD_E_ALIGN;
+    const Plan f = fwd_plan(a.Z, a.KVH, a.R, a.Lk, a.D, p->dtype);
     a.out = out;
     a.lse = lse;
+    a.rest = rest;
     if (f.splits > 1) {
         if (!ws) return NSD_E_NULL;
         if (ws_bytes < (int64_t)(f.splits * state_bytes(a))) return NSD_E_SIZE;
@@ -897,18 +1234,23 @@ extern "C" int nsd_attn_fwd(const void *q, const void *k, const void *v, const N
     }
     if (const int rc = run_fwd<false>(a, f, p->dtype, (hipStream_t)stream)) return rc;
     if (f.splits == 1) return NSD_OK;
-    JoinArgs j{a.po, a.pm, a.pl, f.splits, a.D, a.KVH, a.G, a.Lq, (size_t)a.Z * a.Lq * a.KVH * a.G, nullptr, nullptr, nullptr, out, lse};
+    JoinArgs j{a.po, a.pm, a.pl, f.splits, a.D, a.KVH, a.G, a.Lq, 0, (size_t)a.Z * a.Lq * a.KVH * a.G, nullptr, nullptr, nullptr, out, rest, lse};
     return run_join(j, p->dtype, (hipStream_t)stream);
 }
 
 extern "C" int64_t nsd_attn_bwd_workspace(const NsdSeqAttn *p)
 {
-    if (!p || p->batch < 1 || p->len_q < 1 || p->heads < 1) return 0;
-    return (int64_t)p->batch * p->len_q * p->heads * 4;
+    if (!p || p->batch < 1 || p->len_q < 0 || p->len_k < 0 || p->heads < 1 || p->kv_heads < 1 || p->hd < 1) return 0;
+    const int R = p->len_q * (p->heads / p->kv_heads);
+    const BwdScratch b = bwd_scratch(bwd_q_plan(p->batch, p->kv_heads, R, p->len_k, p->hd, p->dtype),
+                                     bwd_kv_plan(p->batch, p->kv_heads, R, p->len_k, p->hd, p->dtype),
+                                     (size_t)p->batch * p->len_q * p->heads, (size_t)p->batch * p->len_k * p->kv_heads, p->hd);
+    return (int64_t)(b.delta + (b.q > b.kv ? b.q : b.kv));
 }
 
-extern "C" int nsd_attn_bwd(const void *q, const void *k, const void *v, const void *out, const float *lse, const void *dout,
-                            const NsdSeqAttn *p, void *dq, void *dk, void *dv, void *ws, int64_t ws_bytes, void *stream)
+extern "C" int nsd_attn_bwd(const void *q, const void *k, const void *v, const void *out, const float *lse, const int8_t *rest,
+                            const void *dout, const NsdSeqAttn *p, void *dq, void *dk, void *dv, void *ws, int64_t ws_bytes,
+                            void *stream)
 {
     SeqArgs a;
     if (const int rc = seq_args(p, q, k, v, a)) return rc;
@@ -916,19 +1258,23 @@ extern "C" int nsd_attn_bwd(const void *q, const void *k, const void *v, const v
     if (p->batch == 0) return NSD_OK;
     if (a.R > 0 && (!out || !lse || !dout || !dq || !ws)) return NSD_E_NULL;
     if (a.Lk > 0 && (!dk || !dv)) return NSD_E_NULL;
-    if (!al16(out) || !al16(dout) || !al16(dq) || !al16(dk) || !al16(dv) || !al16(ws)) return NSD_E_ALIGN;
-    if (ws_bytes < (int64_t)a.Z * a.KVH * a.R * 4) return NSD_E_SIZE;
+    if (!al16(out) || !al16(rest) || !al16(dout) || !al16(dq) || !al16(dk) || !al16(dv) || !al16(ws)) return NSD_E_ALIGN;
+    const Plan pq = bwd_q_plan(a.Z, a.KVH, a.R, a.Lk, a.D, p->dtype), pk = bwd_kv_plan(a.Z, a.KVH, a.R, a.Lk, a.D, p->dtype);
+    const BwdScratch b = bwd_scratch(pq, pk, (size_t)a.Z * a.KVH * a.R, (size_t)a.Z * a.KVH * a.Lk, a.D);
+    if (ws_bytes < (int64_t)(b.delta + (b.q > b.kv ? b.q : b.kv))) return NSD_E_SIZE;
     a.out = const_cast<void *>(out);
     a.lse = const_cast<float *>(lse);
+    a.rest = const_cast<int8_t *>(rest);
     a.dout = dout;
     a.delta = (float *)ws;
+    a.part = (float *)((char *)ws + b.delta);
     a.dq = dq; a.dk = dk; a.dv = dv;
     if (p->dtype == 0) {
-        if (dp_of(a.D) == 64) launch_bwd<float, 64>(a, (hipStream_t)stream);
-        else launch_bwd<float, 128>(a, (hipStream_t)stream);
+        if (dp_of(a.D) == 64) launch_bwd<float, 64>(a, pq, pk, (hipStream_t)stream);
+        else launch_bwd<float, 128>(a, pq, pk, (hipStream_t)stream);
     } else {
-        if (dp_of(a.D) == 64) launch_bwd<BF16, 64>(a, (hipStream_t)stream);
-        else launch_bwd<BF16, 128>(a, (hipStream_t)stream);
+        if (dp_of(a.D) == 64) launch_bwd<BF16, 64>(a, pq, pk, (hipStream_t)stream);
+        else launch_bwd<BF16, 128>(a, pq, pk, (hipStream_t)stream);
     }
     return (int)hipGetLastError();
 }
@@ -947,10 +1293,8 @@ extern "C" int nsd_attn_prefix(const void *q, const void *k, const void *v, cons
     if (p->batch == 0 || p->len_q == 0) return NSD_OK;
     if (!part_o || !part_m || !part_l) return NSD_E_NULL;
     if (!al16(part_o) || !al16(ws)) return NSD_E_ALIGN;
-    const FwdPlan f = fwd_plan(a.Z, a.KVH, a.R, a.Lk, a.D, p->dtype);
+    const Plan f = fwd_plan(a.Z, a.KVH, a.R, a.Lk, a.D, p->dtype);
     const size_t rows = (size_t)a.Z * a.Lq * a.KVH * a.G;
-    a.splits = f.splits;
-    a.split_tiles = f.split_tiles;
     if (has_state) { a.in_o = part_o; a.in_m = part_m; a.in_l = part_l; }
     a.po = part_o; a.pm = part_m; a.pl = part_l;
     if (f.splits > 1) {
@@ -962,6 +1306,6 @@ extern "C" int nsd_attn_prefix(const void *q, const void *k, const void *v, cons
     }
     if (const int rc = run_fwd<true>(a, f, p->dtype, (hipStream_t)stream)) return rc;
     if (f.splits == 1) return NSD_OK;
-    JoinArgs j{a.po, a.pm, a.pl, f.splits, a.D, a.KVH, a.G, a.Lq, rows, part_o, part_m, part_l, nullptr, nullptr};
+    JoinArgs j{a.po, a.pm, a.pl, f.splits, a.D, a.KVH, a.G, a.Lq, 0, rows, part_o, part_m, part_l, nullptr, nullptr, nullptr};
     return run_join(j, p->dtype, (hipStream_t)stream);
 }

@@ -123,8 +123,8 @@ def load():
     for name in ("nsd_attn_fwd_workspace", "nsd_attn_bwd_workspace", "nsd_attn_prefix_workspace"):
         getattr(L, name).restype = i64
         getattr(L, name).argtypes = [C.POINTER(SeqAttn)]
-    L.nsd_attn_fwd.argtypes = [vp, vp, vp, C.POINTER(SeqAttn), vp, vp, vp, i64, vp]
-    L.nsd_attn_bwd.argtypes = [vp, vp, vp, vp, vp, vp, C.POINTER(SeqAttn), vp, vp, vp, vp, i64, vp]
+    L.nsd_attn_fwd.argtypes = [vp, vp, vp, C.POINTER(SeqAttn), vp, vp, vp, vp, i64, vp]
+    L.nsd_attn_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, C.POINTER(SeqAttn), vp, vp, vp, vp, i64, vp]
     L.nsd_attn_prefix.argtypes = [vp, vp, vp, C.POINTER(SeqAttn), i32, vp, vp, vp, vp, i64, vp]
     for name in EXPORTS:
         getattr(L, name)

@@ -40,19 +40,42 @@ def _same_type(name: str, first: torch.Tensor, *more) -> int:
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # (the stream's handle alone: building a torch.cuda.Stream object costs more than the launch)
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _on:
+    """The tensors' device as the current one, as torch.cuda.device does, but for nothing where it is that already."""
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.prev = torch._C._cuda_getDevice()
+        if self.prev != self.index:
+            torch._C._cuda_setDevice(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch._C._cuda_setDevice(self.prev)
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x, or a copy of it, with consecutive elements in its rows and everything else in steps of 16 bytes."""
+    a, b, c, d = x.stride()
+    n = x.shape
     piece = 16 // x.element_size()
-    ok = (x.stride(-1) == 1 or x.shape[-1] == 1) and x.data_ptr() % 16 == 0 and all(
-        s % piece == 0 or n == 1 for s, n in zip(x.stride()[:-1], x.shape[:-1]))
+    ok = d == 1 and x.data_ptr() % 16 == 0 and (a % piece == 0 or n[0] == 1) and (b % piece == 0 or n[1] == 1) and (
+        c % piece == 0 or n[2] == 1)
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
-def _strides(x: torch.Tensor, *dims: int):
-    return (C.c_int64 * 3)(*(x.stride(d) if x.shape[d] > 1 else 0 for d in dims))
+_I64x3 = C.c_int64 * 3
+
+
+def _strides(x: torch.Tensor, i: int, j: int, k: int):
+    s, n = x.stride(), x.shape                                  # (the stride of an axis of one element says nothing)
+    return _I64x3(s[i] if n[i] > 1 else 0, s[j] if n[j] > 1 else 0, s[k] if n[k] > 1 else 0)
 
 
 def _scratch(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
@@ -80,37 +103,39 @@ class _Attention(torch.autograd.Function):
         q, k, v = _rows(q.detach()), _rows(k.detach()), _rows(v.detach())
         Z, Lq, H, D = q.shape
         L = _lib.load()
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             p = _seq(q, k, v, mask, causal, scale)
-            out = torch.empty(Z, Lq, H, D, dtype=q.dtype, device=q.device)
-            keep = any(ctx.needs_input_grad[:3])
-            lse = torch.empty(Z, k.shape[2], Lq, H // k.shape[2], dtype=torch.float32, device=q.device) if keep else None
-            n = L.nsd_attn_fwd_workspace(C.byref(p))
+            out = torch.empty((Z, Lq, H, D), dtype=q.dtype, device=q.device)
+            lse = rest = None
+            if any(ctx.needs_input_grad):
+                lse = torch.empty((Z, k.shape[2], Lq, H // k.shape[2]), dtype=torch.float32, device=q.device)
+                rest = torch.empty((Z, Lq, H, D), dtype=torch.int8, device=q.device) if p.dtype else None
+            n = L.nsd_attn_fwd_workspace(p)
             ws = _scratch(n, q.device)
-            _lib.check(L.nsd_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), C.byref(p), out.data_ptr(), _ptr(lse),
-                                      _ptr(ws), n, _stream(q.device)), "nsd_attn_fwd")
-        if keep:
-            ctx.save_for_backward(q, k, v, mask, out, lse)
-            ctx.causal, ctx.scale = causal, scale
+            _lib.check(L.nsd_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), p, out.data_ptr(), _ptr(lse),
+                                      _ptr(rest), _ptr(ws), n, _stream(q.device)), "nsd_attn_fwd")
+        if lse is not None:
+            ctx.save_for_backward(q, k, v, mask, out, lse, rest)
+            ctx.shape = p                                       # (the tensors it points at are kept with it)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, mask, out, lse = ctx.saved_tensors
-        L = _lib.load()
-        with torch.cuda.device(q.device):
-            p = _seq(q, k, v, mask, ctx.causal, ctx.scale)
+        q, k, v, mask, out, lse, rest = ctx.saved_tensors
+        L, p = _lib.load(), ctx.shape
+        with _on(q.device):
             dout = dout.contiguous()
             if dout.data_ptr() % 16:
                 dout = dout.clone()
             dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
-            n = L.nsd_attn_bwd_workspace(C.byref(p))
+            dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+            dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+            n = L.nsd_attn_bwd_workspace(p)
             ws = _scratch(n, q.device)
-            _lib.check(L.nsd_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                                      dout.data_ptr(), C.byref(p), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws),
-                                      n, _stream(q.device)), "nsd_attn_bwd")
+            _lib.check(L.nsd_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _ptr(rest),
+                                      dout.data_ptr(), p, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), n,
+                                      _stream(q.device)), "nsd_attn_bwd")
         return dq, dk, dv, None, None, None
 
 
@@ -186,7 +211,7 @@ def shared_prefix_attention(q: torch.Tensor, prefixes: Sequence, kgen: torch.Ten
     if not 0.0 < scale < math.inf:
         raise ValueError("shared_prefix_attention: scale is a positive number")
     L, dev = _lib.load(), q.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         st = _stream(dev)
         q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
         out = torch.empty_like(q)
@@ -200,13 +225,13 @@ def shared_prefix_attention(q: torch.Tensor, prefixes: Sequence, kgen: torch.Ten
             s = _lib.SeqAttn()
             s.batch, s.len_q, s.len_k, s.heads, s.kv_heads, s.hd, s.dtype = n, M // n, k.shape[2], H, KVH, D, dt
             s.scale = scale
-            s.q_stride = (C.c_int64 * 3)(M // n * H * D, H * D, D)
+            s.q_stride = _I64x3(M // n * H * D, H * D, D)
             s.k_stride, s.v_stride = _strides(k, 0, 2, 1), _strides(v, 0, 2, 1)
             lens = p[2].contiguous() if len(p) == 3 else None
             s.key_len = _ptr(lens)
-            nb = L.nsd_attn_prefix_workspace(C.byref(s))
+            nb = L.nsd_attn_prefix_workspace(s)
             ws = _scratch(nb, dev)
-            _lib.check(L.nsd_attn_prefix(q.data_ptr(), k.data_ptr(), v.data_ptr(), C.byref(s), int(i > 0), po, pm, pl,
+            _lib.check(L.nsd_attn_prefix(q.data_ptr(), k.data_ptr(), v.data_ptr(), s, int(i > 0), po, pm, pl,
                                          _ptr(ws), nb, st), "nsd_attn_prefix")
         part = (po, pm, pl) if state is not None else (None, None, None)
         _lib.check(L.nsd_attn_step(q.data_ptr(), None, None, kgen.data_ptr(), vgen.data_ptr(), _ptr(anc), out.data_ptr(),
@@ -223,7 +248,7 @@ class _AddRmsNorm(torch.autograd.Function):
         xc, wc = _flat(x.detach()), _flat(w.detach())
         dc = None if delta is None else _flat(delta.detach())
         L = _lib.load()
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
             x_out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if dc is not None else None
             _lib.check(L.nsd_add_rmsnorm(xc.data_ptr(), _ptr(dc), wc.data_ptr(), eps, x.numel() // hidden, hidden,
@@ -243,7 +268,7 @@ class _AddRmsNorm(torch.autograd.Function):
             dx, dw = dx_out, torch.zeros_like(w) if want_w else None
         else:
             L = _lib.load()
-            with torch.cuda.device(x_out.device):
+            with _on(x_out.device):
                 dh = _flat(dh)
                 go = None if dx_out is None else _flat(dx_out)
                 dx = torch.empty(x_out.shape, dtype=x_out.dtype, device=x_out.device)
@@ -271,6 +296,8 @@ def add_rms_norm(x: torch.Tensor, delta: Optional[torch.Tensor], w: torch.Tensor
         raise ValueError("add_rms_norm takes x and delta [..., hidden] and w [hidden]")
     _same_device("add_rms_norm", x, delta, w)
     dt = _same_type("add_rms_norm", x, delta, w)
+    if x.numel() // max(1, x.shape[-1]) >= 2 ** 31:
+        raise ValueError("add_rms_norm: at most 2^31 - 1 rows")
     if x.shape[-1] < 1 or x.shape[-1] % (8 if dt else 4):
         raise ValueError(f"add_rms_norm: hidden = {x.shape[-1]} is not a multiple of {8 if dt else 4}")
     return _AddRmsNorm.apply(x, delta, w, float(eps))

@@ -285,22 +285,22 @@ def _seq(**kw):
 def test_c_entries_refuse_what_they_cannot_do():
     lib, L = _lib()
     A, SIZE, NULL = 4096, -7, -1                                 # an aligned address that no refused call reads
-    fwd = lambda p, q=A, k=A, v=A, out=A, ws=None, n=0: L.nsd_attn_fwd(q, k, v, C.byref(p), out, None, ws, n, None)   # noqa: E731
+    fwd = lambda p, q=A, k=A, v=A, out=A, ws=None, n=0: L.nsd_attn_fwd(q, k, v, C.byref(p), out, None, None, ws, n, None)   # noqa: E731
     for bad in (dict(hd=4), dict(hd=136), dict(hd=60), dict(heads=3), dict(heads=0), dict(kv_heads=0), dict(dtype=2), dict(scale=0.0),
                 dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(batch=-1), dict(len_q=-1), dict(len_k=-2),
                 dict(len_q=1 << 30, heads=8), dict(batch=1 << 30), dict(len_k=(1 << 30) + 1)):
         assert fwd(_seq(**bad)) == SIZE, bad
-        assert L.nsd_attn_bwd(A, A, A, A, A, A, C.byref(_seq(**bad)), A, A, A, A, 1 << 40, None) == SIZE, bad
+        assert L.nsd_attn_bwd(A, A, A, A, A, None, A, C.byref(_seq(**bad)), A, A, A, A, 1 << 40, None) == SIZE, bad
         assert L.nsd_attn_prefix(A, A, A, C.byref(_seq(**{"causal": 0, **bad})), 0, A, A, A, A, 1 << 40, None) == SIZE, bad
     assert fwd(_seq(), q=None) == NULL and fwd(_seq(), k=None) == NULL and fwd(_seq(), out=None) == NULL
     for bad in ("q_stride", "k_stride", "v_stride"):
         assert fwd(_seq(**{bad: (1024, 250, 64)})) == lib.E_ALIGN
     assert fwd(_seq(), q=A + 8) == lib.E_ALIGN and fwd(_seq(), out=A + 2) == lib.E_ALIGN
     assert fwd(_seq(batch=0)) == 0 and fwd(_seq(len_q=0)) == 0    # nothing to do
-    long = _seq(len_q=1, len_k=5000)
+    long = _seq(len_q=1, len_k=50000)
     need = L.nsd_attn_fwd_workspace(C.byref(long))
     assert need > 0 and fwd(long) == NULL and fwd(long, ws=A, n=need - 1) == SIZE
-    bwd = lambda p, ws=A, n=1 << 20, dq=A, dk=A: L.nsd_attn_bwd(A, A, A, A, A, A, C.byref(p), dq, dk, A, ws, n, None)   # noqa: E731
+    bwd = lambda p, ws=A, n=1 << 20, dq=A, dk=A: L.nsd_attn_bwd(A, A, A, A, A, None, A, C.byref(p), dq, dk, A, ws, n, None)   # noqa: E731
     assert bwd(_seq(), ws=None) == NULL and bwd(_seq(), n=8) == SIZE and bwd(_seq(), dq=None) == NULL and bwd(_seq(), dk=A + 4) == lib.E_ALIGN
     p = _seq()
     p.key_len = A
