@@ -413,22 +413,22 @@ typedef struct NsdSeqAttn {
 /* out [batch, len_q, heads, hd] = softmax(scale q k^T over the visible keys) v; a row that sees no key is zeros.
  *   lse  fp32 [batch, kv_heads, len_q, heads / kv_heads] or NULL: the natural logarithm of each row's sum of
  *        exponentials (-inf for a row that sees no key), what nsd_attn_bwd recomputes the probabilities from
- *   rest int8 [batch, len_q, heads, hd] or NULL (always NULL for fp32): what rounding to bf16 took from out, in 256ths
- *        of out's last place, from which nsd_attn_bwd has its row sums of dout x out to 16 bits of out
+ *   rest u8 [batch, len_q, heads, hd] or NULL (always NULL for fp32): 128 + what rounding to bf16 took from out, in
+ *        256ths of out's last place, from which nsd_attn_bwd has its row sums of dout x out to 16 bits of out
  *   ws   device scratch of nsd_attn_fwd_workspace(p) bytes (may be NULL where that is 0), free again when the
  *        stream has passed the call; NSD_E_SIZE if ws_bytes is less
  * Results do not depend on anything but the arguments (no atomics; the split of the keys over workgroups is a
  * function of the sizes).  Replaces the attention of the frozen LLM's layers (train_emg_llm.py:145-181). */
 int64_t nsd_attn_fwd_workspace(const NsdSeqAttn *p);
 int nsd_attn_fwd(const void *q, const void *k, const void *v, const NsdSeqAttn *p, void *out, float *lse,
-                 int8_t *rest, void *ws, int64_t ws_bytes, void *stream);
+                 uint8_t *rest, void *ws, int64_t ws_bytes, void *stream);
 
 /* Gradients of that attention for dout [batch, len_q, heads, hd]; out, lse and rest (or NULL) as nsd_attn_fwd left
  * them.
  *   dq [batch, len_q, heads, hd], dk, dv [batch, len_k, kv_heads, hd] (summed over the query heads of a kv head);
  *   zeros for masked keys and for rows that see no key.  ws: nsd_attn_bwd_workspace(p) bytes. */
 int64_t nsd_attn_bwd_workspace(const NsdSeqAttn *p);
-int nsd_attn_bwd(const void *q, const void *k, const void *v, const void *out, const float *lse, const int8_t *rest,
+int nsd_attn_bwd(const void *q, const void *k, const void *v, const void *out, const float *lse, const uint8_t *rest,
                  const void *dout, const NsdSeqAttn *p, void *dq, void *dk, void *dv, void *ws, int64_t ws_bytes, void *stream);
 
 /* Softmax state of a beam step over keys that hypotheses share, each key read once for all of them; any number of

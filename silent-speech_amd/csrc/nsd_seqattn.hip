@@ -23,6 +23,8 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -174,37 +176,45 @@ NSD_D void store4(BF16 *p, float a, float b, float c, float d)
     *reinterpret_cast<uint2 *>(p) = make_uint2(u, w);
 }
 
-// What rounding to bf16 took from v, in 256ths of the last place that bf16 keeps: a signed byte, with which the row sums
-// dO . O of the backward pass see 16 bits of O.  (With bf16's 8 alone the error of dQ and dK grows by up to 1.3 times, at
-// short rows; the whole rest in bf16 costs 13 us of traffic in a training step of 8 x 640 positions, the byte half of it.)
-NSD_D float pow2_of(BF16 v) { return __uint_as_float((uint32_t)(v.b & 0x7f80u) << 16); }
-NSD_D int rest_of(float v)
-{
-    const BF16 r = from_f<BF16>(v);
-    const float inv = __uint_as_float(0x7f000000u - ((uint32_t)(r.b & 0x7f80u) << 16));
-    return (int)fminf(fmaxf(__builtin_rintf((v - to_f(r)) * inv * 32768.0f), -127.0f), 127.0f);
-}
+// What rounding to bf16 took from a value, in 256ths of the last place that bf16 keeps, plus 128: a byte, with which the
+// row sums dO . O of the backward pass see 16 bits of O.  (With bf16's 8 alone the error of dQ and dK grows by up to 1.3
+// times, most at short rows; the rest in bf16 is twice the traffic.)
 NSD_D uint32_t rest4(float a, float b, float c, float d)
 {
-    return (uint32_t)(rest_of(a) & 255) | (uint32_t)(rest_of(b) & 255) << 8 | (uint32_t)(rest_of(c) & 255) << 16 | (uint32_t)rest_of(d) << 24;
+    const float v[4] = {a, b, c, d};
+    uint32_t r = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+        const f32x2 x = {v[j], v[j + 1]};
+        const uint32_t u = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t hi = i ? u & 0xffff0000u : u << 16;
+            // 2^15 / 2^exponent; a value below 2^-111 has no rest
+            const float inv = __uint_as_float(max(0x7f000000u + (15u << 23) - max(hi & 0x7f800000u, 16u << 23), 0u));
+            r = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_fmaf(v[j + i] - __uint_as_float(hi), inv, 128.0f), j + i, r);
+        }
+    }
+    return r;
 }
 // sum of g times the rest of o over a lane's eight elements
-NSD_D float rest_dot(const Frag<BF16> &g, const Frag<BF16> &o, const int8_t *rest, float s)
+NSD_D float rest_dot(const Frag<BF16> &g, const Frag<BF16> &o, const uint8_t *rest, float s)
 {
     const uint2 c = *reinterpret_cast<const uint2 *>(rest);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const int8_t b = (int8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
-        const float f = pow2_of(__builtin_bit_cast(BF16, (__bf16)o.v[j]));
-        s = __builtin_fmaf((float)g.v[j], (float)b * f * (1.0f / 32768.0f), s);
+        const float b = (float)((j < 4 ? c.x : c.y) >> (8 * (j & 3)) & 255u) - 128.0f;
+        const float f = __uint_as_float(__float_as_uint((float)o.v[j]) & 0x7f800000u);
+        s = __builtin_fmaf((float)g.v[j] * f, b * (1.0f / 32768.0f), s);
     }
     return s;
 }
-NSD_D float rest_dot(const Frag<float> &, const Frag<float> &, const int8_t *, float s) { return s; }
+NSD_D float rest_dot(const Frag<float> &, const Frag<float> &, const uint8_t *, float s) { return s; }
 
 // A wave's 32 rows from its transposed accumulators (lane = row, registers = elements) to memory, times `mul`.  bf16 rows
 // pass through LDS (`s`, the wave's own 32 * (RB + 16) bytes) and leave in 16-byte pieces of whole rows: stored from the
-// accumulators they would be 8 bytes here and there, 16 stores that touch 32 rows each.  ptr(r) is row r's place or null.
+// accumulators they would be 8 bytes here and there, 16 stores that touch 32 rows each.  The stores pass by the caches,
+// which the keys need (32 x 768 positions: 212 -> 187 us).  ptr(r) is row r's place or null.
 template <class T, int DP, class P>
 NSD_D void put_rows(char *s, const f32x16 (&o)[DP / 32], float mul, int D, int lane, P ptr)
 {
@@ -222,7 +232,8 @@ NSD_D void put_rows(char *s, const f32x16 (&o)[DP / 32], float mul, int D, int l
         for (int i = 0; i < 32 * PR / 64; ++i) {
             const int r = (i * 64 + lane) / PR, p = (i * 64 + lane) % PR;
             T *dst = ptr(r);
-            if (dst && p * 8 < D) *reinterpret_cast<uint4 *>(dst + p * 8) = *reinterpret_cast<const uint4 *>(s + r * SB + p * 16);
+            if (dst && p * 8 < D)
+                __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(s + r * SB + p * 16), reinterpret_cast<u32x4 *>(dst + p * 8));
         }
         nsd_wave_sync();
     } else {
@@ -253,8 +264,9 @@ NSD_D void put_rest(char *s, const f32x16 (&o)[DP / 32], float mul, int D, int l
 #pragma unroll
     for (int i = 0; i < 32 * PR / 64; ++i) {
         const int r = (i * 64 + lane) / PR, p = (i * 64 + lane) % PR;
-        int8_t *dst = ptr(r);
-        if (dst && p * 8 < D) *reinterpret_cast<uint2 *>(dst + p * 8) = *reinterpret_cast<const uint2 *>(s + r * SB + p * 8);
+        uint8_t *dst = ptr(r);
+        if (dst && p * 8 < D)
+            __builtin_nontemporal_store(*reinterpret_cast<const u32x2 *>(s + r * SB + p * 8), reinterpret_cast<u32x2 *>(dst + p * 8));
     }
 }
 
@@ -272,7 +284,7 @@ struct SeqArgs {
     // forward
     void *out;                             // [Z, Lq, heads, D]
     float *lse;                            // [Z, KVH, R], natural logarithm
-    int8_t *rest;                          // a byte for each element of out, or null: see rest_of
+    uint8_t *rest;                         // a byte for each element of out, or null: see rest4
     float *po, *pm, *pl;                   // state [splits][Z * Lq * heads] (sum of weighted values, maximum, sum)
     const float *in_o, *in_m, *in_l;       // a state to continue, or null
     int splits, split_tiles, batch;
@@ -386,7 +398,7 @@ template <class T, int DP, int ROWS> struct Stage {
 // BN = KW * WN each; their states meet at the end).  grid.x = row tile, (z, kv head), split.
 // ---------------------------------------------------------------------
 template <class T, int DP, int WM, int KW, int NBUF, bool STATE>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 && NBUF * KW / WM * DP <= 4096 ? 2 : 1)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && 2 * NBUF * KW * (4 / WM) * DP * 2 <= 81920 ? 2 : 1)
 nsd_attn_fwd_kernel(SeqArgs a)
 {
     constexpr int WN = 4 / WM, BM = 32 * WM, BN = KW * WN, NK = KW / 32, DT = DP / 32, KC = DP / 16;
@@ -608,7 +620,7 @@ struct JoinArgs {
     size_t rows;
     float *so, *sm, *sl;
     void *out;
-    int8_t *rest;
+    uint8_t *rest;
     float *lse;
 };
 
@@ -696,7 +708,7 @@ nsd_attn_sum_kernel(const float *part, size_t n, int splits, T *out)
 // the second part.  Layout of the forward: a wave owns 32 rows, S^T and dP^T are computed from the same tiles.
 // ---------------------------------------------------------------------
 template <class T, int DP, int WM, int NK, int NBUF>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && 2 * NBUF * 32 * NK * (4 / WM) * DP * 2 <= 81920 ? 2 : 1)
 nsd_attn_bwd_q_kernel(SeqArgs a)
 {
     constexpr int WN = 4 / WM, BM = 32 * WM, BN = 32 * NK * WN, DT = DP / 32, KC = DP / 16;
@@ -844,7 +856,7 @@ nsd_attn_bwd_q_kernel(SeqArgs a)
 // rows at the same time.
 // ---------------------------------------------------------------------
 template <class T, int DP, int WK, int NS, int NBUF>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && 2 * NBUF * 32 * NS * (4 / WK) * DP * 2 <= 81920 ? 2 : 1)
 nsd_attn_bwd_kv_kernel(SeqArgs a)
 {
     constexpr int WR = 4 / WK, BN = 32 * WK, BM = 32 * WR * NS, DT = DP / 32, KC = DP / 16;
@@ -1212,7 +1224,7 @@ extern "C" int64_t nsd_attn_fwd_workspace(const NsdSeqAttn *p)
     return f.splits > 1 ? (int64_t)f.splits * p->batch * p->len_q * p->heads * (p->hd + 2) * 4 : 0;
 }
 
-extern "C" int nsd_attn_fwd(const void *q, const void *k, const void *v, const NsdSeqAttn *p, void *out, float *lse, int8_t *rest,
+extern "C" int nsd_attn_fwd(const void *q, const void *k, const void *v, const NsdSeqAttn *p, void *out, float *lse, uint8_t *rest,
                             void *ws, int64_t ws_bytes, void *stream)
 {
     SeqArgs a;
@@ -1248,7 +1260,7 @@ extern "C" int64_t nsd_attn_bwd_workspace(const NsdSeqAttn *p)
     return (int64_t)(b.delta + (b.q > b.kv ? b.q : b.kv));
 }
 
-extern "C" int nsd_attn_bwd(const void *q, const void *k, const void *v, const void *out, const float *lse, const int8_t *rest,
+extern "C" int nsd_attn_bwd(const void *q, const void *k, const void *v, const void *out, const float *lse, const uint8_t *rest,
                             const void *dout, const NsdSeqAttn *p, void *dq, void *dk, void *dv, void *ws, int64_t ws_bytes,
                             void *stream)
 {
@@ -1264,7 +1276,7 @@ extern "C" int nsd_attn_bwd(const void *q, const void *k, const void *v, const v
     if (ws_bytes < (int64_t)(b.delta + (b.q > b.kv ? b.q : b.kv))) return NSD_E_SIZE;
     a.out = const_cast<void *>(out);
     a.lse = const_cast<float *>(lse);
-    a.rest = const_cast<int8_t *>(rest);
+    a.rest = const_cast<uint8_t *>(rest);
     a.dout = dout;
     a.delta = (float *)ws;
     a.part = (float *)((char *)ws + b.delta);

@@ -109,7 +109,7 @@ class _Attention(torch.autograd.Function):
             lse = rest = None
             if any(ctx.needs_input_grad):
                 lse = torch.empty((Z, k.shape[2], Lq, H // k.shape[2]), dtype=torch.float32, device=q.device)
-                rest = torch.empty((Z, Lq, H, D), dtype=torch.int8, device=q.device) if p.dtype else None
+                rest = torch.empty((Z, Lq, H, D), dtype=torch.uint8, device=q.device) if p.dtype else None
             n = L.nsd_attn_fwd_workspace(p)
             ws = _scratch(n, q.device)
             _lib.check(L.nsd_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), p, out.data_ptr(), _ptr(lse),
