@@ -6,8 +6,12 @@ hypothesis at a time and keeps the last position (inference_emg_llm.py:427-429).
 prompt embeddings, EMG adapter output) is run once per utterance and its keys/values are shared by the
 utterance's hypotheses; every step then feeds ONE new token per hypothesis, after re-ordering the cache of the
 generated positions by the scorer's back-pointers.  `teacher_logits` scores whole candidate transcripts against the
-same cached contexts in one causal pass (the `ar_logprob` of eval_ar.py:574-588).  The dense contractions stay torch / hipBLASLt; this module
-is plumbing around them (no hand-written kernels), and its output feeds `NSDecoder.step`.
+same cached contexts in one causal pass (the `ar_logprob` of eval_ar.py:574-588).  A prompt that all utterances share
+(soft prompt + prompt embeddings) may be given apart, as `prefix`: `HipLlamaStep` then keeps one copy of its keys / values
+and every step reads them once for all hypotheses.  `train_logits` is the teacher-forced forward pass of training
+(train_emg_llm.py:145-181), differentiable.  The dense contractions stay torch / hipBLASLt; `TorchLlamaStep` is plumbing
+around them (no hand-written kernels), `HipLlamaStep` has the library's kernels between them; the output feeds
+`NSDecoder.step`.
 
 Architecture = transformers' LlamaModel (pre-norm, RMSNorm, rotary embedding in the rotate-half form, grouped
 query attention, SwiGLU MLP, final norm) + `char_embed` + `lm_head`; `from_hf` takes the weights of such a
@@ -68,6 +72,7 @@ class TorchLlamaStep:
         self.inv_freq = inv.to(self.device)
         self.scale = 1.0 / math.sqrt(dims.head_dim)
         self.N = self.B = self.S = self.T = 0
+        self.P = 0                                      # positions of a prefix kept apart from the contexts
 
     # ------------------------------------------------------------------ weights
     def _random_weights(self, seed: int) -> dict:
@@ -122,6 +127,35 @@ class TorchLlamaStep:
         return (q.unflatten(-1, (d.heads, d.head_dim)), k.unflatten(-1, (d.kv_heads, d.head_dim)),
                 v.unflatten(-1, (d.kv_heads, d.head_dim)))
 
+    # what differs between the two implementations in a pass over whole sequences; q, k, v [Z, positions, heads, hd]
+    def _add_norm(self, x: torch.Tensor, delta: Optional[torch.Tensor], w: torch.Tensor):
+        x = x if delta is None else x + delta
+        return x, _rms(x, w, self.d.rms_eps)
+
+    def _attention(self, q, k, v, key_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Causal, the last query sees the last key; key_mask [Z, keys]."""
+        Lq, Lk = q.shape[1], k.shape[1]
+        mask = torch.ones(Lq, Lk, dtype=torch.bool, device=q.device).tril(Lk - Lq)
+        if key_mask is not None:
+            mask = mask & key_mask[:, None, None, :]
+        q, k, v = (x.transpose(1, 2) for x in (q, k, v))
+        return F.scaled_dot_product_attention(q, k, v, attn_mask=mask, enable_gqa=True).transpose(1, 2)
+
+    def _layers(self, x: torch.Tensor, pos0: int, attend) -> torch.Tensor:
+        """The decoder layers and the final norm over x [Z, positions, hidden], whose first row is at position pos0;
+        attend(l, q, k, v) is layer l's attention, of rotated q and k."""
+        d = self.d
+        cos, sin = self._cos_sin(pos0 + torch.arange(x.shape[1], device=self.device))
+        cos, sin = cos[None, :, None, :], sin[None, :, None, :]
+        delta = None
+        for l in range(d.layers):
+            x, h = self._add_norm(x, delta, self.w[f"{l}.ln1"])
+            q, k, v = self._split_qkv(F.linear(h, self.w[f"{l}.qkv"]))
+            a = attend(l, _rope(q, cos, sin), _rope(k, cos, sin), v)
+            x, h = self._add_norm(x, F.linear(a.flatten(-2), self.w[f"{l}.o"]), self.w[f"{l}.ln2"])
+            delta = self._mlp(l, h)
+        return self._add_norm(x, delta, self.w["norm"])[1]
+
     def _mlp(self, l: int, x: torch.Tensor) -> torch.Tensor:
         gu = F.linear(x, self.w[f"{l}.gate_up"])
         g, u = gu.split(self.d.intermediate, dim=-1)
@@ -129,11 +163,15 @@ class TorchLlamaStep:
 
     # ------------------------------------------------------------------ context (prefill)
     @torch.no_grad()
-    def encode_context(self, context: torch.Tensor, beam: int, max_new_tokens: int) -> None:
+    def encode_context(self, context: torch.Tensor, beam: int, max_new_tokens: int,
+                       prefix: Optional[torch.Tensor] = None) -> None:
         """context [N, S, hidden] (soft prompt + prompt embeddings + EMG adapter output, what
-        EMGTextModel.encode_context returns): one causal pass; keys/values are kept per utterance."""
+        EMGTextModel.encode_context returns): one causal pass; keys/values are kept per utterance.
+        prefix [P, hidden]: rows in front of every utterance's context (here simply joined to each)."""
         d = self.d
         x = context.to(self.device, self.dtype)
+        if prefix is not None:
+            x = torch.cat((prefix.to(x).expand(x.shape[0], -1, -1), x), dim=1)
         N, S, _ = x.shape
         self.N, self.B, self.S, self.T = N, int(beam), S, int(max_new_tokens)
         M = N * self.B
@@ -261,6 +299,34 @@ class TorchLlamaStep:
         x = _rms(x, self.w["norm"], d.rms_eps)
         return F.linear(x, self.w["lm_head.w"], self.w["lm_head.b"]).float()
 
+    # ------------------------------------------------------------------ training forward
+    def train_logits(self, context: torch.Tensor, in_ids: torch.Tensor, context_len: Optional[torch.Tensor] = None,
+                     prefix: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Teacher-forced logits for the cross entropy (train_emg_llm.py:145-181): one causal pass over
+        [prefix ; context ; char_embed(in_ids)] per utterance, row i = logits after in_ids[:, :i+1].
+
+        context [N, S, hidden], in_ids [N, L] integer (padded with any valid id), context_len [N]: real rows of a
+        padded context, at least one (default all), the others are seen by no position; prefix [P, hidden] (soft prompt
+        + prompt embeddings).  Returns float32 [N, L, vocab], differentiable in context, prefix and whatever entry of
+        `self.w` requires a gradient (the reference trains char_embed and lm_head, the layers stay frozen)."""
+        x = context.to(self.device, self.dtype)
+        N, S, _ = x.shape
+        in_ids = in_ids.to(self.device).long()
+        L = in_ids.shape[1]
+        mask = None
+        if context_len is not None:
+            if tuple(context_len.shape) != (N,):
+                raise ValueError("context_len is [N]")
+            mask = torch.arange(S, device=self.device)[None] < context_len.to(self.device)[:, None]
+            mask = torch.cat((mask, mask.new_ones(N, L)), dim=1)
+        x = torch.cat((x, F.embedding(in_ids, self.w["char_embed"])), dim=1)
+        if prefix is not None:
+            x = torch.cat((prefix.to(x).expand(N, -1, -1), x), dim=1)
+            if mask is not None:
+                mask = torch.cat((mask.new_ones(N, prefix.shape[0]), mask), dim=1)
+        h = self._layers(x, 0, lambda l, q, k, v: self._attention(q, k, v, mask))[:, x.shape[1] - L:]
+        return F.linear(h, self.w["lm_head.w"], self.w["lm_head.b"]).float()
+
     # ------------------------------------------------------------------ glue for NSDecoder.decode_batch
     def step_fn_batched(self):
         return self._step_fn_batched()
@@ -283,12 +349,18 @@ class HipLlamaStep(TorchLlamaStep):
     """The same step with everything between the dense contractions in HIP kernels of libnsdecode.so
     (nsd_add_rmsnorm, nsd_rope_kv_append, nsd_attn_step, nsd_swiglu) and a generated-position cache that is never
     re-ordered: position s is a slab [M, kv_heads, hd] written once, and a hypothesis reads the slab rows of its
-    ancestors, found through the scorer's back-pointer array (nsd_ancestors).  GPU only."""
+    ancestors, found through the scorer's back-pointer array (nsd_ancestors).  GPU only.
+
+    With a `prefix`, or with long_context=True, whole sequences and the shared part of a step's attention go through
+    nsd_attn_fwd / nsd_attn_prefix: any number of prefix and context positions, fp32 or bf16, each key read once for
+    the hypotheses that share it (nsd_attn_ctx does that for up to 256 bf16 positions; past it the per-hypothesis kernel
+    reads the context again for every hypothesis).  Both sum the same terms in another order."""
 
     _DT = {torch.float32: 0, torch.bfloat16: 1}
 
-    def __init__(self, *a, use_mfma: bool = True, **kw):
+    def __init__(self, *a, use_mfma: bool = True, long_context: bool = False, **kw):
         super().__init__(*a, **kw)
+        self.long_context = bool(long_context)
         self.use_mfma = bool(use_mfma)
         if self.dtype not in self._DT:
             raise ValueError("HipLlamaStep stores fp32 or bf16")
@@ -297,11 +369,30 @@ class HipLlamaStep(TorchLlamaStep):
         from . import lib as _lib
         self._lib, self._L = _lib, _lib.load()
 
+    def _add_norm(self, x, delta, w):
+        from . import ops
+        return ops.add_rms_norm(x, delta, w, self.d.rms_eps)
+
+    def _attention(self, q, k, v, key_mask=None):
+        from . import ops
+        return ops.attention(q, k, v, key_mask=key_mask, scale=self.scale)
+
     @torch.no_grad()
-    def encode_context(self, context: torch.Tensor, beam: int, max_new_tokens: int) -> None:
-        super().encode_context(context, beam, max_new_tokens)
-        d, M, T = self.d, self.N * self.B, max(self.T, 1)
-        del self.kg, self.vg
+    def encode_context(self, context: torch.Tensor, beam: int, max_new_tokens: int,
+                       prefix: Optional[torch.Tensor] = None) -> None:
+        """As TorchLlamaStep.encode_context; the keys / values of `prefix` [P, hidden] are computed and kept once."""
+        d = self.d
+        self.levels = None                                       # per layer: what nsd_attn_prefix reads
+        if prefix is not None or self.long_context:
+            if d.head_dim not in (8, 16, 32, 64, 128):
+                raise ValueError("a prefix or a long context needs a head dimension of 8, 16, 32, 64 or 128")
+            self._prefill(context, prefix)
+            self.B, self.T, self.t = int(beam), int(max_new_tokens), 0
+        else:
+            self.P = 0
+            super().encode_context(context, beam, max_new_tokens)
+            del self.kg, self.vg
+        M, T = self.N * self.B, max(self.T, 1)
         kw = dict(dtype=self.dtype, device=self.device)
         self.kgen = torch.zeros(d.layers, T, M, d.kv_heads, d.head_dim, **kw)
         self.vgen = torch.zeros(d.layers, T, M, d.kv_heads, d.head_dim, **kw)
@@ -312,7 +403,7 @@ class HipLlamaStep(TorchLlamaStep):
         # multiple of 32 rows, values transposed; per query row the softmax state the per-hypothesis kernel continues
         S32 = (self.S + 31) // 32 * 32
         self.mfma_ctx = (self.dtype == torch.bfloat16 and d.head_dim in (64, 128) and 0 < self.S and S32 <= 256
-                         and self.use_mfma)
+                         and self.use_mfma and self.levels is None)
         if self.mfma_ctx:
             self.S32 = S32
             self.kpad, self.vt = [], []
@@ -326,6 +417,57 @@ class HipLlamaStep(TorchLlamaStep):
             self.part_o = torch.empty(M * d.heads, d.head_dim, dtype=torch.float32, device=self.device)
             self.part_m = torch.empty(M * d.heads, dtype=torch.float32, device=self.device)
             self.part_l = torch.empty(M * d.heads, dtype=torch.float32, device=self.device)
+
+    def _prefill(self, context: torch.Tensor, prefix: Optional[torch.Tensor]) -> None:
+        x = context.to(self.device, self.dtype)
+        self.N, self.S, _ = x.shape
+        self.P = 0
+        self.kp, self.vp, self.levels = [], [], []
+        kpre, vpre = [], []
+
+        def keep(l, q, k, v):
+            kpre.append(k.contiguous())
+            vpre.append(v.contiguous())
+            return self._attention(q, k, v)
+
+        def attend(l, q, k, v):
+            own = (k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous())
+            self.kp.append(own[0])
+            self.vp.append(own[1])
+            self.levels.append([own] if self.S else [])
+            if self.P:
+                self.levels[l].insert(0, (kpre[l].transpose(1, 2), vpre[l].transpose(1, 2)))
+                k, v = (torch.cat((a.expand(self.N, -1, -1, -1), b), dim=1) for a, b in ((kpre[l], k), (vpre[l], v)))
+            return self._attention(q, k, v)
+
+        if prefix is not None and prefix.shape[0]:
+            self._layers(prefix.to(x)[None], 0, keep)
+            self.P = prefix.shape[0]
+        self._layers(x, self.P, attend)
+
+    @torch.no_grad()
+    def teacher_logits(self, seq: torch.Tensor, lens: torch.Tensor, utt: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if self.N == 0 or self.levels is None:
+            return super().teacher_logits(seq, lens, utt)
+        seq = seq.to(self.device).long()
+        M, L = seq.shape
+        if L < 2:
+            return torch.zeros(M, 0, self.d.vocab, dtype=torch.float32, device=self.device)
+        utt = torch.arange(M, device=self.device) % self.N if utt is None else utt.to(self.device).long()
+
+        def attend(l, q, k, v):
+            # [prefix ; the utterance's context ; the sequence]
+            levels = [x for x in self.levels[l]]
+            parts = []
+            if self.P:
+                parts.append([x.transpose(1, 2).expand(M, -1, -1, -1) for x in levels.pop(0)])
+            if levels:
+                parts.append([x.transpose(1, 2).index_select(0, utt) for x in levels[0]])
+            k, v = (torch.cat([p[i] for p in parts] + [x], dim=1) for i, x in ((0, k), (1, v)))
+            return self._attention(q, k, v)
+
+        h = self._layers(F.embedding(seq[:, :L - 1], self.w["char_embed"]), self.P + self.S, attend)
+        return F.linear(h, self.w["lm_head.w"], self.w["lm_head.b"]).float()
 
     def _tmp(self, name, *shape):
         b = self._buf.get(name)
@@ -353,7 +495,7 @@ class HipLlamaStep(TorchLlamaStep):
                 self._own_bp[t - 1] = backptr
                 backptr_all = self._own_bp
             lib.check(L.nsd_ancestors(backptr_all.data_ptr(), t, N, B, self.anc.data_ptr(), st), "nsd_ancestors")
-        ang = (S + t) * self.inv_freq
+        ang = (self.P + S + t) * self.inv_freq
         ang = torch.cat((ang, ang))
         if self.dtype == torch.float32:
             cos, sin = ang.cos().contiguous(), ang.sin().contiguous()
@@ -373,15 +515,20 @@ class HipLlamaStep(TorchLlamaStep):
             lib.check(L.nsd_rope_kv_append(qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), M, d.heads, d.kv_heads,
                                            d.head_dim, dt, q.data_ptr(), self.kgen[l, t].data_ptr(),
                                            self.vgen[l, t].data_ptr(), st), "nsd_rope_kv_append")
+            if self.levels is not None:
+                from . import ops
+                att = ops.shared_prefix_attention(q, self.levels[l], self.kgen[l], self.vgen[l], self.anc, t, B,
+                                                  scale=self.scale).view(M, -1)
             po = pm = pl = None
             if self.mfma_ctx:
                 po, pm, pl = self.part_o.data_ptr(), self.part_m.data_ptr(), self.part_l.data_ptr()
                 lib.check(L.nsd_attn_ctx(q.data_ptr(), self.kpad[l].data_ptr(), self.vt[l].data_ptr(), N, B, d.heads,
                                          d.kv_heads, d.head_dim, S, self.S32, self.scale, po, pm, pl, st), "nsd_attn_ctx")
-            lib.check(L.nsd_attn_step(q.data_ptr(), self.kp[l].data_ptr(), self.vp[l].data_ptr(),
-                                      self.kgen[l].data_ptr(), self.vgen[l].data_ptr(), self.anc.data_ptr(),
-                                      att.data_ptr(), N, B, d.heads, d.kv_heads, d.head_dim, S, t, self.scale, dt,
-                                      po, pm, pl, st), "nsd_attn_step")
+            if self.levels is None:
+                lib.check(L.nsd_attn_step(q.data_ptr(), self.kp[l].data_ptr(), self.vp[l].data_ptr(),
+                                          self.kgen[l].data_ptr(), self.vgen[l].data_ptr(), self.anc.data_ptr(),
+                                          att.data_ptr(), N, B, d.heads, d.kv_heads, d.head_dim, S, t, self.scale, dt,
+                                          po, pm, pl, st), "nsd_attn_step")
             o = F.linear(att, self.w[f"{l}.o"])
             lib.check(L.nsd_add_rmsnorm(x.data_ptr(), o.data_ptr(), self.w[f"{l}.ln2"].data_ptr(), d.rms_eps, M,
                                         d.hidden, dt, x.data_ptr(), h.data_ptr(), st), "nsd_add_rmsnorm")

@@ -372,3 +372,175 @@ def test_swiglu_kernel(dtype, rows, inter):
     tol = 3e-6 if dtype == torch.float32 else 1.6e-2
     err = (out.float() - want).abs() / want.abs().clamp(min=1.0)
     assert float(err.max()) <= tol
+
+
+# ---------------------------------------------------------------------- shared prefixes, long contexts, training
+def _small_head(kind, dims, device, dtype=torch.float32, seed=3, **kw):
+    from silent_speech_amd import ar_head
+    w = ar_head.TorchLlamaStep(dims, dtype=dtype, device="cpu", seed=seed).w
+    # weights of a size that lets attention and norms matter (the random initialisation is nearly linear)
+    w = {k: (v * 4 if k.split(".")[-1] in ("qkv", "o", "gate_up", "down") else v).clone() for k, v in w.items()}
+    g = torch.Generator().manual_seed(seed)
+    w = {k: v + 0.2 * torch.randn(v.shape, generator=g).to(v) if ".ln" in k or k == "norm" else v for k, v in w.items()}
+    return getattr(ar_head, kind)(dims, dtype=dtype, device=device, weights=w, **kw)
+
+
+def _small_dims(**kw):
+    from silent_speech_amd.ar_head import LlamaDims
+    return LlamaDims(**{**dict(hidden=64, layers=2, heads=6, kv_heads=2, head_dim=16, intermediate=96), **kw})
+
+
+def test_prefix_equals_the_joined_context_cpu():
+    """A prefix in front of every context is the same as contexts that start with it."""
+    dims = _small_dims()
+    g = torch.Generator().manual_seed(1)
+    prefix, ctx = torch.randn(5, 64, generator=g), torch.randn(3, 7, 64, generator=g)
+    a, b = (_small_head("TorchLlamaStep", dims, "cpu") for _ in range(2))
+    a.encode_context(ctx, 2, 3, prefix=prefix)
+    b.encode_context(torch.cat((prefix.expand(3, -1, -1), ctx), 1), 2, 3)
+    tok = torch.full((6,), 37)
+    assert torch.equal(a.step(tok), b.step(tok))
+
+
+def test_train_logits_against_the_reference_formulation_cpu():
+    """train_logits and its gradients against transformers' LlamaModel over [context ; char_embed(ids)] with a key mask,
+    fp32, padded contexts; the cached teacher-forced rows say the same."""
+    llm, char_embed, lm_head = _reference_setup(2)
+    from silent_speech_amd.ar_head import TorchLlamaStep
+    head = TorchLlamaStep.from_hf(llm, char_embed.weight.data, lm_head.weight.data, lm_head.bias.data, dtype=torch.float32, device="cpu")
+    N, S, L = 3, 8, 5
+    torch.manual_seed(4)
+    ctx = (torch.randn(N, S, 64) * 0.5).requires_grad_()
+    ids = torch.randint(0, 37, (N, L))
+    lens = torch.tensor([8, 5, 1])
+    for n in ("char_embed", "lm_head.w", "lm_head.b"):
+        head.w[n].requires_grad_()
+    got = head.train_logits(ctx, ids, lens)
+    mask = torch.cat((torch.arange(S)[None] < lens[:, None], torch.ones(N, L, dtype=torch.bool)), 1)
+    full = torch.ones(S + L, S + L, dtype=torch.bool).tril()[None, None] & mask[:, None, None]
+    bias = torch.zeros(full.shape).masked_fill(~full, torch.finfo(torch.float32).min)
+    for p in llm.parameters():
+        p.requires_grad_(False)
+    h = llm(inputs_embeds=torch.cat((ctx, char_embed(ids)), 1), attention_mask=bias).last_hidden_state[:, S:]
+    want = lm_head(h)
+    assert float((got - want).detach().abs().max()) < 2e-4
+    go = torch.randn(N, L, 40)
+    mine = torch.autograd.grad(got, (ctx, head.w["char_embed"], head.w["lm_head.w"], head.w["lm_head.b"]), go)
+    ref = torch.autograd.grad(want, (ctx, char_embed.weight, lm_head.weight, lm_head.bias), go)
+    for i, (x, y) in enumerate(zip(mine, ref)):
+        assert float((x - y).abs().max()) < 5e-4 * max(1.0, float(y.abs().max())), i
+    head.encode_context(ctx.detach()[:1], 1, 4)
+    teacher = head.teacher_logits(torch.cat((ids[:1], ids[:1, :1]), 1), torch.tensor([L + 1]))
+    assert float((teacher - got[:1]).detach().abs().max()) < 2e-4
+
+
+def _train_grads(head, ctx, ids, out_ids, lens, prefix, tables):
+    """One training step's loss (cross entropy + 0.05 x the LM regulariser) and the gradients of what it trains."""
+    from silent_speech_amd.prior import ns_lm_regularizer
+    ctx, prefix = (x.to(head.device).requires_grad_() for x in (ctx, prefix))
+    names = ("char_embed", "lm_head.w", "lm_head.b")
+    for n in names:
+        head.w[n] = head.w[n].detach().requires_grad_()
+    logits = head.train_logits(ctx, ids, lens, prefix=prefix)
+    loss = torch.nn.functional.cross_entropy(logits.flatten(0, 1), out_ids.to(head.device).flatten(), ignore_index=-100)
+    loss = loss + 0.05 * ns_lm_regularizer(logits, ids, out_ids.to(head.device), tables)
+    grads = torch.autograd.grad(loss, (ctx, prefix, *(head.w[n] for n in names)))
+    return [loss.detach(), logits.detach(), *grads]
+
+
+def _train_case(dims, N=3, S=21, P=6, L=9, seed=8):
+    from oracle import ns_oracle as O, synth
+    from silent_speech_amd.prior import tables_from_lm
+    g = torch.Generator().manual_seed(seed)
+    words = synth.make_lexicon(40, 3, max_len=5)
+    tables = tables_from_lm(O.NgramLM(3, floor_vsz=True).fit(synth.make_sentences(words, 300, 1)))
+    ids = torch.randint(0, 37, (N, L), generator=g)
+    out = torch.cat((ids[:, 1:], torch.full((N, 1), 38)), 1)
+    out[0, 4:] = -100
+    return (torch.randn(N, S, dims.hidden, generator=g), ids, out, torch.tensor([S, S // 3, 2][:N]), torch.randn(P, dims.hidden, generator=g), tables)
+
+
+@pytest.mark.gpu
+def test_hip_training_step_equals_torch():
+    """A training step through the library's attention, norms and regulariser against the torch-only head: loss, logits
+    and the gradients of the context, the prompt, char_embed and lm_head.
+
+    fp32: every value of a gradient is a sum over a few thousand products of values that two layers' fp32 sums of a
+    hundred to a thousand terms produced, in another order on the two sides: relative differences of 1e3 x 2^-24 = 6e-5
+    of the largest value, doubled by a second layer and the softmaxes: 2e-4.
+    bf16: both sides round some 20 tensors on the way from a gradient to the context, and the torch side the attention's
+    weights too, each off by up to 2^-9 on average of the values' size; errors of 20 independent roundings on two sides
+    add up to sqrt(40) 2^-9 = 1.3e-2 of a tensor's norm; 4e-2 holds three times that."""
+    for dtype, tol in ((torch.float32, 2e-4), (torch.bfloat16, 4e-2)):
+        dims = _small_dims(hidden=128, head_dim=64, intermediate=160)
+        case = _train_case(dims)
+        a = _train_grads(_small_head("TorchLlamaStep", dims, "cuda", dtype), *case)
+        b = _train_grads(_small_head("HipLlamaStep", dims, "cuda", dtype), *case)
+        for i, (x, y) in enumerate(zip(a, b)):
+            x, y = x.double(), y.double()
+            if dtype == torch.float32:
+                assert float((x - y).abs().max()) <= tol * max(float(x.abs().max()), 1e-3), (dtype, i)
+            else:
+                assert float((x - y).norm()) <= tol * float(x.norm()), (dtype, i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("P,S,long_context", [(6, 9, False), (300, 40, False), (0, 70, True), (130, 0, False), (3, 290, True)])
+def test_hip_decode_over_a_shared_prefix_equals_torch(P, S, long_context):
+    """Steps and teacher-forced rows over [prefix shared by all ; context ; generated], fp32, against the torch-only
+    head with joined contexts, through re-ordered beams; tolerance as for the other step tests."""
+    dims = _small_dims()
+    a, b = _small_head("TorchLlamaStep", dims, "cuda"), _small_head("HipLlamaStep", dims, "cuda", long_context=long_context)
+    N, B, T = 3, 5, 6
+    g = torch.Generator().manual_seed(P + S)
+    prefix = torch.randn(P, dims.hidden, generator=g) if P else None
+    ctx = torch.randn(N, S, dims.hidden, generator=g)
+    a.encode_context(ctx, B, T, prefix=prefix)
+    b.encode_context(ctx, B, T, prefix=prefix)
+    tok, bp = torch.full((N * B,), 37, dtype=torch.int64, device="cuda"), None
+    for t in range(T):
+        la, lb = a.step(tok, backptr=bp), b.step(tok, backptr=bp)
+        assert float((la - lb).abs().max()) < 2e-4 * max(1.0, float(la.abs().max())), t
+        bp = torch.randint(0, B, (N * B,), generator=g, dtype=torch.uint8).cuda()
+        tok = torch.randint(0, 37, (N * B,), generator=g).cuda()
+    seq = torch.randint(0, 37, (2 * N, 7), generator=g)
+    lens = torch.full((2 * N,), 7)
+    la, lb = a.teacher_logits(seq, lens), b.teacher_logits(seq, lens)
+    assert float((la - lb).abs().max()) < 2e-4 * max(1.0, float(la.abs().max()))
+
+
+@pytest.mark.gpu
+def test_hip_decode_batch_with_a_shared_prompt():
+    """The scorer's whole loop over a prompt that all utterances share: the same transcripts and scores as from contexts
+    that each start with it (fp32; a step's logits agree to 2e-4, scores are sums of up to 10 of their log-softmax)."""
+    from oracle import ns_oracle as O, synth
+    from silent_speech_amd.decoder import DeviceTables, NSDecoder
+    dims = _small_dims()
+    words = synth.make_lexicon(60, 3, max_len=6)
+    tables = DeviceTables.from_words(words, O.NgramLM(3, floor_vsz=False).fit(synth.make_sentences(words, 500, 1)))
+    N, B, T = 5, 4, 10
+    g = torch.Generator().manual_seed(9)
+    prefix, ctx = torch.randn(40, dims.hidden, generator=g), torch.randn(N, 12, dims.hidden, generator=g)
+    got = []
+    for kind, joined in (("HipLlamaStep", False), ("HipLlamaStep", True)):
+        head = _small_head(kind, dims, "cuda")
+        head.w["lm_head.w"] = head.w["lm_head.w"] * 30.0        # logits of order 1: the beam has preferences
+        if joined:
+            head.encode_context(torch.cat((prefix.expand(N, -1, -1), ctx), 1), B, T)
+        else:
+            head.encode_context(ctx, B, T, prefix=prefix)
+        dec = NSDecoder(tables, B, T, variant="I", lm_weight=0.3, oov_penalty=1.0)
+        got.append(dec.decode_batch(head.step_fn_batched(), N, needs_ids=False, check_every=0))
+    (ia, la, sa), (ib, lb, sb) = got
+    assert float((sa - sb).abs().max()) < 1e-2
+    assert torch.equal(la, lb) and all(torch.equal(ia[u, :la[u]], ib[u, :lb[u]]) for u in range(N))
+
+
+@pytest.mark.gpu
+def test_prefix_refuses_a_head_dimension_it_cannot_read():
+    dims = _small_dims(head_dim=256)
+    head = _small_head("HipLlamaStep", dims, "cuda")
+    with pytest.raises(ValueError):
+        head.encode_context(torch.zeros(1, 3, 64), 2, 2, prefix=torch.zeros(2, 64))
+    with pytest.raises(ValueError):
+        head.train_logits(torch.zeros(1, 3, 64, device="cuda"), torch.zeros(1, 2, dtype=torch.long))
