@@ -264,6 +264,146 @@ def test_add_rms_norm_of_no_rows_and_odd_views():
     assert torch.equal(a[1], b[1])
 
 
+# ---------------------------------------------------------------------- streams, graphs, threads
+def _work(seed, L=150, dtype=BF):
+    g = _gen(seed)
+    KVH, G, D = 2, 3, 64
+    x = [torch.randn(2, L, h, D, generator=g).to(dtype).cuda() for h in (KVH * G, KVH, KVH)]
+    do = torch.randn(2, L, KVH * G, D, generator=g).to(dtype).cuda()
+    r = [torch.randn(300, 256, generator=g).to(dtype).cuda() for _ in range(4)]
+    w = torch.randn(256, generator=g).to(dtype).cuda()
+    q, ps, kgen, vgen, anc = _beam_case(dtype, 2, 6, 2, 2, 64, [(1, 1300, None), (2, 50, [50, 7])], 3, seed)
+    beam = (q.cuda(), [tuple(y.cuda() for y in p) for p in ps], kgen.cuda(), vgen.cuda(), anc.cuda(), 3, 6)
+    return x, do, r, w, beam
+
+
+def _all_ops(x, do, r, w, beam):
+    """Every operator once, forward and backward, from leaves of its own."""
+    from silent_speech_amd import ops
+    leaves = [y.detach().requires_grad_() for y in x]
+    out = ops.attention(*leaves)
+    got = [out, *torch.autograd.grad(out, leaves, do)]
+    ln = [y.detach().requires_grad_() for y in (r[0], r[1], w)]
+    x_out, h = ops.add_rms_norm(*ln)
+    got += [x_out, h, *torch.autograd.grad((x_out, h), ln, (r[2], r[3]))]
+    got.append(ops.shared_prefix_attention(*beam))
+    return [y.detach() for y in got]
+
+
+@pytest.mark.gpu
+def test_operators_give_the_same_bits_again_and_on_other_streams():
+    case = _work(1)
+    want = [y.clone() for y in _all_ops(*case)]
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(_all_ops(*case), want))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for st in streams:                                          # two at once, their scratch apart
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            got.append([_all_ops(*case) for _ in range(5)])
+    for st in streams:
+        torch.cuda.current_stream().wait_stream(st)
+    for runs in got:
+        for run in runs:
+            assert all(torch.equal(a, b) for a, b in zip(run, want))
+
+
+@pytest.mark.gpu
+def test_operators_in_two_captured_graphs():
+    """Forward and backward passes captured into two graphs, replayed by turns with other inputs and the program's own
+    eager work between: every replay equals the eager result."""
+    cases = [_work(2, 150), _work(3, 90)]
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for c in cases:
+            _all_ops(*c)
+    torch.cuda.current_stream().wait_stream(side)
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(_all_ops(*c))
+        graphs.append(g)
+    for i in range(4):
+        for c in cases:                                         # new inputs in the captured places
+            for t in (*c[0], c[1], *c[2], c[4][0]):
+                t.copy_(torch.randn(t.shape, generator=_gen(100 + i)).to(t.dtype))
+        want = [[y.clone() for y in _all_ops(*c)] for c in cases]
+        for k in (0, 1, 0):
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        for o, e in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(o, e)), i
+
+
+@pytest.mark.gpu
+def test_operators_from_two_threads():
+    import threading
+    cases = [_work(5, 120), _work(6, 77)]
+    want = [[y.clone() for y in _all_ops(*c)] for c in cases]
+    bad = []
+
+    def run(i):
+        try:
+            st = torch.cuda.Stream()
+            st.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(st):
+                runs = [_all_ops(*cases[i]) for _ in range(20)]
+            st.synchronize()
+            if not all(torch.equal(a, b) for r in runs for a, b in zip(r, want[i])):
+                bad.append(i)
+        except Exception as e:                                  # noqa: BLE001 - reported below
+            bad.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    torch.cuda.synchronize()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+@pytest.mark.gpu
+def test_gradients_are_differentiable_once():
+    from silent_speech_amd import ops
+    q, k, v = (torch.randn(1, 9, 2, 32, device="cuda").requires_grad_() for _ in range(3))
+    (dq,) = torch.autograd.grad(ops.attention(q, k, v).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dq.sum().backward()
+    x, w = torch.randn(3, 32, device="cuda").requires_grad_(), torch.ones(32, device="cuda")
+    (dx,) = torch.autograd.grad(ops.add_rms_norm(x, None, w)[1].sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
+@pytest.mark.gpu
+def test_attention_over_an_offset_past_32_bits():
+    """Keys and values more than 4 GiB apart within one call: the batch stride of a large cache."""
+    from silent_speech_amd import ops
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GiB")
+    g = _gen(4)
+    L, D = 130, 64
+    far = (1 << 31) + (1 << 20)                                 # elements: 4.3 GB
+    base = torch.empty(far + L * D, dtype=BF, device="cuda")
+    k = base.as_strided((2, L, 1, D), (far, D, D, 1))
+    k.copy_(torch.randn(2, L, 1, D, generator=g).to(BF))
+    q = torch.randn(2, L, 2, D, generator=g).to(BF).cuda()
+    want = ops.attention(q, k.contiguous(), k.contiguous())
+    assert torch.equal(ops.attention(q, k, k), want)
+    tok = base.as_strided((1, 2, 1, D), (0, far, D, 1))         # the same as a position's stride
+    ref = ops.attention(q[:1, :2], tok.contiguous(), tok.contiguous())
+    assert torch.equal(ops.attention(q[:1, :2], tok, tok), ref)
+    kgen = torch.zeros(1, 4, 1, D, dtype=BF, device="cuda")
+    pre = base.as_strided((2, 1, L, D), (far, D, D, 1))
+    qs = torch.randn(4, 2, D, generator=g).to(BF).cuda()
+    a, b = (ops.shared_prefix_attention(qs, [(p, p)], kgen, kgen, None, 0, 2) for p in (pre, pre.contiguous()))
+    assert torch.equal(a, b)
+
+
 # ---------------------------------------------------------------------- refusals (no GPU needed)
 def _lib():
     from silent_speech_amd import lib
