@@ -64,6 +64,16 @@ NSD_D Frag<float> acc_frag(const f32x16 &s, int c, float)
     return f;
 }
 
+// what that rounding left of them, as an operand of its own: with both, a product sees 16 bits of the accumulator
+NSD_D Frag<BF16> rest_frag(const f32x16 &s, int c, const Frag<BF16> &hi)
+{
+    f32x16 r = s;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[8 * c + j] = s[8 * c + j] - (float)hi.v[j];
+    return acc_frag(r, c, BF16{});
+}
+NSD_D Frag<float> rest_frag(const f32x16 &, int, const Frag<float> &f) { return f; }
+
 NSD_D float half_max(float v)
 {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -717,6 +727,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && 2 * NBUF * 32 * NK * (4
 nsd_attn_bwd_q_kernel(SeqArgs a)
 {
     constexpr int WN = 4 / WM, BM = 32 * WM, BN = 32 * NK * WN, DT = DP / 32, KC = DP / 16;
+    // where workgroups are few and the launch waits on latencies, dS enters its product with 16 bits instead of 8: the
+    // error of dQ against 64 bits is then 1.1 instead of 1.4 times that of one rounding, for nothing
+    constexpr bool FINE = sizeof(T) == 2 && WM == 1;
     constexpr int NW = BN > 64 ? BN / 64 : 1;
     using TL = Tile<T, DP>;
     constexpr int TB = BN * TL::RB;
@@ -816,9 +829,13 @@ nsd_attn_bwd_q_kernel(SeqArgs a)
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const Frag<T> p = acc_frag(s, c, T{});
+                const Frag<T> p = acc_frag(s, c, T{}), rest = rest_frag(s, c, p);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) mma(o[dt], TL::col_frag(sk, kw0 + 32 * n + 16 * c, dt, lane), p);
+                for (int dt = 0; dt < DT; ++dt) {
+                    const Frag<T> k = TL::col_frag(sk, kw0 + 32 * n + 16 * c, dt, lane);
+                    mma(o[dt], k, p);
+                    if constexpr (FINE) mma(o[dt], k, rest);
+                }
             }
         }
     }
@@ -865,6 +882,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && 2 * NBUF * 32 * NS * (4
 nsd_attn_bwd_kv_kernel(SeqArgs a)
 {
     constexpr int WR = 4 / WK, BN = 32 * WK, BM = 32 * WR * NS, DT = DP / 32, KC = DP / 16;
+    constexpr bool FINE = sizeof(T) == 2 && WK == 1;            // as in the first part
     using TL = Tile<T, DP>;
     constexpr int TB = BM * TL::RB;
     static_assert(WR == 1 || 2 * NBUF * TB >= 4 * 32 * DP * 4, "the waves' sums meet in the tiles' place");
@@ -982,6 +1000,14 @@ nsd_attn_bwd_kv_kernel(SeqArgs a)
                     mma(dv[dt], TL::col_frag(sg, 32 * n + 16 * c, dt, lane), p);
                     mma(dk[dt], TL::col_frag(sq, 32 * n + 16 * c, dt, lane), ds);
                 }
+                if constexpr (FINE) {
+                    const Frag<T> p_rest = rest_frag(s, c, p), ds_rest = rest_frag(dp, c, ds);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        mma(dv[dt], TL::col_frag(sg, 32 * n + 16 * c, dt, lane), p_rest);
+                        mma(dk[dt], TL::col_frag(sq, 32 * n + 16 * c, dt, lane), ds_rest);
+                    }
+                }
             }
 
         }
@@ -1071,7 +1097,7 @@ Plan bwd_q_plan(int Z, int KVH, int R, int Lk, int D, int dtype)
 {
     Plan p;
     const int64_t pairs = (int64_t)Z * KVH;
-    p.wave_rows = pairs * div_up(R, 128) >= CUS ? 4 : pairs * div_up(R, 64) >= CUS ? 2 : 1;
+    p.wave_rows = R > 64 && pairs * div_up(R, 128) >= CUS ? 4 : R > 32 && pairs * div_up(R, 64) >= CUS ? 2 : 1;
     p.bn = p.wave_rows == 4 ? (dtype == 0 && dp_of(D) == 128 ? 32 : 64) : 32 * (4 / p.wave_rows);
     p.tiles = (int)div_up(R, 32 * p.wave_rows);
     split_walk(p, p.tiles * pairs, div_up(Lk, p.bn), CUS, dtype == 0 ? 1 : 8);
@@ -1085,7 +1111,7 @@ Plan bwd_kv_plan(int Z, int KVH, int R, int Lk, int D, int dtype)
 {
     Plan p;
     const int64_t pairs = (int64_t)Z * KVH;
-    p.wave_rows = pairs * div_up(Lk, 64) >= CUS / 2 ? 2 : 1;       // (waves along the keys here)
+    p.wave_rows = Lk > 32 && pairs * div_up(Lk, 64) >= CUS / 2 ? 2 : 1;     // (waves along the keys here)
     p.bn = 32 * p.wave_rows;
     p.tiles = (int)div_up(Lk, p.bn);
     split_walk(p, p.tiles * pairs, div_up(R, 32 * (4 / p.wave_rows)), CUS, dtype == 0 ? 1 : 8);
