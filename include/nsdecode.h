@@ -354,8 +354,8 @@ int nsd_add_rmsnorm(const void *x, const void *delta, const void *w, float eps, 
  * dx_out of x_out (NULL: x_out is not used elsewhere), with x_out as the forward stored it,
  *   dx = dx_out + r (g - xh mean(g xh)),  r = rsqrt(mean(x_out^2) + eps), xh = x_out r, g = dh w:
  * the gradient of x and of delta alike; dw (NULL: not wanted) = sum over the rows of dh xh.  Arrays in the element
- * type, sums in fp32 and in a fixed order; the rounding of xh inside the forward is passed through.  dx may be dx_out
- * or dh.  ws: nsd_add_rmsnorm_bwd_workspace bytes of device scratch, needed where dw is. */
+ * type, sums in fp32 and in a fixed order; the rounding of xh inside the forward is passed through.  dx may be dx_out.
+ * ws: nsd_add_rmsnorm_bwd_workspace bytes of device scratch, needed where dw is. */
 int64_t nsd_add_rmsnorm_bwd_workspace(int32_t rows, int32_t hidden);
 int nsd_add_rmsnorm_bwd(const void *x_out, const void *w, const void *dh, const void *dx_out, float eps, int32_t rows,
                         int32_t hidden, int32_t dtype, void *dx, void *dw, void *ws, int64_t ws_bytes, void *stream);
@@ -415,8 +415,8 @@ typedef struct NsdSeqAttn {
  *        exponentials (-inf for a row that sees no key), what nsd_attn_bwd recomputes the probabilities from
  *   rest u8 [batch, len_q, heads, hd] or NULL (always NULL for fp32): 128 + what rounding to bf16 took from out, in
  *        256ths of out's last place, from which nsd_attn_bwd has its row sums of dout x out to 16 bits of out
- *   ws   device scratch of nsd_attn_fwd_workspace(p) bytes (may be NULL where that is 0), free again when the
- *        stream has passed the call; NSD_E_SIZE if ws_bytes is less
+ *   ws   device scratch of nsd_attn_fwd_workspace(p) bytes (may be NULL where that is 0; 0 for a shape that is
+ *        refused), free again when the stream has passed the call; NSD_E_SIZE if ws_bytes is less
  * Results do not depend on anything but the arguments (no atomics; the split of the keys over workgroups is a
  * function of the sizes).  Replaces the attention of the frozen LLM's layers (train_emg_llm.py:145-181). */
 int64_t nsd_attn_fwd_workspace(const NsdSeqAttn *p);

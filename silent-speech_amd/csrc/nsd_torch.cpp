@@ -103,7 +103,7 @@ variable_list once(variable_list grads, const char *name)
     if (!at::GradMode::is_enabled()) return grads;
     auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " is differentiable once", (int)grads.size());
     for (auto &g : grads)
-        if (g.defined()) g.requires_grad_();
+        if (g.defined()) g = g.detach().requires_grad_();
     return (*error)(std::move(grads));
 }
 

@@ -35,6 +35,9 @@ CASES = [  # dtype, Z, Lq, Lk, kv heads, G, hd, causal, mask
     (BF, 2, 1, 700, 2, 4, 128, True, None), (BF, 1, 7, 1000, 1, 3, 64, False, "pad"), (BF, 1, 40, 513, 1, 1, 128, True, "random"),
     (BF, 2, 90, 40, 1, 2, 64, True, None), (BF, 1, 257, 127, 2, 1, 128, False, None), (BF, 1, 20, 64, 1, 5, 24, False, None),
     (BF, 1, 600, 600, 2, 3, 128, True, "random"),
+    # walks split over workgroups: keys of the forward pass and of dQ, rows of dK and dV
+    (BF, 1, 3, 2100, 2, 2, 128, True, "random"), (BF, 1, 50, 3000, 1, 1, 64, False, "pad"), (BF, 1, 600, 600, 1, 8, 64, True, "pad"),
+    (BF, 1, 400, 700, 1, 12, 128, True, "random"), (BF, 2, 9, 40, 1, 32, 64, True, None),
     (FP, 2, 37, 37, 2, 2, 16, True, "pad"), (FP, 1, 130, 130, 1, 3, 64, True, None), (FP, 1, 70, 150, 2, 2, 128, True, "random"),
     (FP, 3, 50, 50, 1, 3, 80, True, "empty"), (FP, 1, 3, 900, 2, 2, 128, False, None), (FP, 1, 33, 700, 1, 2, 64, True, "pad"),
     (FP, 1, 20, 300, 1, 3, 128, False, "random"), (FP, 2, 80, 33, 1, 4, 40, True, None), (FP, 1, 260, 260, 1, 1, 128, False, None),
@@ -182,7 +185,7 @@ def _beam_case(dtype, N, B, KVH, G, D, levels, t, seed):
     (BF, 1, 1, 1, 1, 64, [(1, 1, None)], 0), (BF, 1, 4, 2, 2, 64, [(1, 100, None)], 3), (BF, 2, 5, 2, 3, 128, [(1, 65, None)], 7),
     (BF, 3, 7, 1, 3, 128, [(1, 300, None), (3, 40, None)], 5), (BF, 4, 16, 2, 3, 128, [(1, 1500, None)], 2),
     (BF, 5, 3, 1, 8, 32, [(5, 90, [90, 0, 1, 64, 33])], 4), (BF, 2, 16, 1, 4, 128, [(2, 700, [700, 129])], 1),
-    (BF, 3, 2, 1, 1, 8, [(3, 20, [0, 0, 0])], 0), (BF, 2, 8, 1, 2, 64, [(1, 0, None), (2, 77, None)], 2), (BF, 2, 3, 1, 2, 64, [], 2),
+    (BF, 3, 2, 1, 1, 8, [(3, 20, [0, 0, 0])], 0), (BF, 2, 3, 1, 3, 64, [(2, 90, [-3, 95])], 1), (BF, 2, 8, 1, 2, 64, [(1, 0, None), (2, 77, None)], 2), (BF, 2, 3, 1, 2, 64, [], 2),
     (BF, 6, 4, 1, 3, 64, [(1, 128, None), (2, 64, [64, 5]), (6, 33, None)], 3), (BF, 40, 4, 1, 1, 64, [(1, 70, None)], 2),
     (FP, 1, 4, 2, 2, 64, [(1, 100, None)], 3), (FP, 5, 7, 1, 2, 64, [(5, 150, [150, 3, 0, 149, 70])], 6),
     (FP, 2, 9, 1, 3, 128, [(1, 400, None), (2, 33, [33, 1])], 2), (FP, 2, 12, 1, 2, 128, [(1, 90, None)], 0), (FP, 12, 8, 1, 2, 16, [(1, 40, None)], 1),
@@ -377,6 +380,25 @@ def test_gradients_are_differentiable_once():
     (dx,) = torch.autograd.grad(ops.add_rms_norm(x, None, w)[1].sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         dx.sum().backward()
+    go = torch.ones(3, 32, device="cuda")                       # a gradient that only passes through is left as it was
+    torch.autograd.grad(ops.add_rms_norm(x, None, w)[0], x, go, create_graph=True)
+    assert not go.requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,hidden", [(9, 512), (5, 16392)])
+def test_add_rmsnorm_bwd_writes_over_dx_out(rows, hidden):
+    lib, L = _lib()
+    g = _gen(hidden)
+    x, dh, go = (torch.randn(rows, hidden, generator=g).to(BF).cuda() for _ in range(3))
+    w, dw = torch.randn(hidden, generator=g).to(BF).cuda(), torch.zeros(hidden, dtype=BF, device="cuda")
+    n = L.nsd_add_rmsnorm_bwd_workspace(rows, hidden)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    want = R.add_rms_norm(x, None, w, 1e-5, go, dh)
+    lib.check(L.nsd_add_rmsnorm_bwd(x.data_ptr(), w.data_ptr(), dh.data_ptr(), go.data_ptr(), 1e-5, rows, hidden, 1, go.data_ptr(),
+                                    dw.data_ptr(), ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream), "nsd_add_rmsnorm_bwd")
+    R.within(go, want["dx"], "dx")
+    R.within(dw, want["dw"], "dw")
 
 
 @pytest.mark.gpu
@@ -428,10 +450,12 @@ def test_c_entries_refuse_what_they_cannot_do():
     fwd = lambda p, q=A, k=A, v=A, out=A, ws=None, n=0: L.nsd_attn_fwd(q, k, v, C.byref(p), out, None, None, ws, n, None)   # noqa: E731
     for bad in (dict(hd=4), dict(hd=136), dict(hd=60), dict(heads=3), dict(heads=0), dict(kv_heads=0), dict(dtype=2), dict(scale=0.0),
                 dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(batch=-1), dict(len_q=-1), dict(len_k=-2),
-                dict(len_q=1 << 30, heads=8), dict(batch=1 << 30), dict(len_k=(1 << 30) + 1)):
+                dict(len_q=1 << 30, heads=8), dict(batch=1 << 30), dict(len_k=(1 << 30) + 1),
+                dict(batch=(1 << 31) - 1, heads=1 << 20, kv_heads=1 << 20), dict(len_q=1 << 16, heads=512, kv_heads=1)):
         assert fwd(_seq(**bad)) == SIZE, bad
         assert L.nsd_attn_bwd(A, A, A, A, A, None, A, C.byref(_seq(**bad)), A, A, A, A, 1 << 40, None) == SIZE, bad
         assert L.nsd_attn_prefix(A, A, A, C.byref(_seq(**{"causal": 0, **bad})), 0, A, A, A, A, 1 << 40, None) == SIZE, bad
+        assert L.nsd_attn_fwd_workspace(C.byref(_seq(**bad))) == 0 and L.nsd_attn_bwd_workspace(C.byref(_seq(**bad))) == 0
     assert fwd(_seq(), q=None) == NULL and fwd(_seq(), k=None) == NULL and fwd(_seq(), out=None) == NULL
     for bad in ("q_stride", "k_stride", "v_stride"):
         assert fwd(_seq(**{bad: (1024, 250, 64)})) == lib.E_ALIGN
