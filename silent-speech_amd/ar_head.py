@@ -127,6 +127,11 @@ class TorchLlamaStep:
         return (q.unflatten(-1, (d.heads, d.head_dim)), k.unflatten(-1, (d.kv_heads, d.head_dim)),
                 v.unflatten(-1, (d.kv_heads, d.head_dim)))
 
+    def _prefix_rows(self, prefix: Optional[torch.Tensor], x: torch.Tensor) -> Optional[torch.Tensor]:
+        if prefix is not None and (prefix.dim() != 2 or prefix.shape[1] != self.d.hidden):
+            raise ValueError(f"prefix is [P, {self.d.hidden}]")
+        return None if prefix is None else prefix.to(x)
+
     # what differs between the two implementations in a pass over whole sequences; q, k, v [Z, positions, heads, hd]
     def _add_norm(self, x: torch.Tensor, delta: Optional[torch.Tensor], w: torch.Tensor):
         x = x if delta is None else x + delta
@@ -170,8 +175,9 @@ class TorchLlamaStep:
         prefix [P, hidden]: rows in front of every utterance's context (here simply joined to each)."""
         d = self.d
         x = context.to(self.device, self.dtype)
+        prefix = self._prefix_rows(prefix, x)
         if prefix is not None:
-            x = torch.cat((prefix.to(x).expand(x.shape[0], -1, -1), x), dim=1)
+            x = torch.cat((prefix.expand(x.shape[0], -1, -1), x), dim=1)
         N, S, _ = x.shape
         self.N, self.B, self.S, self.T = N, int(beam), S, int(max_new_tokens)
         M = N * self.B
@@ -320,8 +326,9 @@ class TorchLlamaStep:
             mask = torch.arange(S, device=self.device)[None] < context_len.to(self.device)[:, None]
             mask = torch.cat((mask, mask.new_ones(N, L)), dim=1)
         x = torch.cat((x, F.embedding(in_ids, self.w["char_embed"])), dim=1)
+        prefix = self._prefix_rows(prefix, x)
         if prefix is not None:
-            x = torch.cat((prefix.to(x).expand(N, -1, -1), x), dim=1)
+            x = torch.cat((prefix.expand(N, -1, -1), x), dim=1)
             if mask is not None:
                 mask = torch.cat((mask.new_ones(N, prefix.shape[0]), mask), dim=1)
         h = self._layers(x, 0, lambda l, q, k, v: self._attention(q, k, v, mask))[:, x.shape[1] - L:]
@@ -420,6 +427,7 @@ class HipLlamaStep(TorchLlamaStep):
 
     def _prefill(self, context: torch.Tensor, prefix: Optional[torch.Tensor]) -> None:
         x = context.to(self.device, self.dtype)
+        prefix = self._prefix_rows(prefix, x)
         self.N, self.S, _ = x.shape
         self.P = 0
         self.kp, self.vp, self.levels = [], [], []
@@ -441,7 +449,7 @@ class HipLlamaStep(TorchLlamaStep):
             return self._attention(q, k, v)
 
         if prefix is not None and prefix.shape[0]:
-            self._layers(prefix.to(x)[None], 0, keep)
+            self._layers(prefix[None], 0, keep)
             self.P = prefix.shape[0]
         self._layers(x, self.P, attend)
 

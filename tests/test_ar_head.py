@@ -400,6 +400,11 @@ def test_prefix_equals_the_joined_context_cpu():
     b.encode_context(torch.cat((prefix.expand(3, -1, -1), ctx), 1), 2, 3)
     tok = torch.full((6,), 37)
     assert torch.equal(a.step(tok), b.step(tok))
+    for bad in (prefix[None], prefix[:, :32], prefix[0]):
+        with pytest.raises(ValueError):
+            a.encode_context(ctx, 2, 3, prefix=bad)
+        with pytest.raises(ValueError):
+            a.train_logits(ctx, torch.zeros(3, 2, dtype=torch.long), prefix=bad)
 
 
 def test_train_logits_against_the_reference_formulation_cpu():
@@ -542,5 +547,7 @@ def test_prefix_refuses_a_head_dimension_it_cannot_read():
     head = _small_head("HipLlamaStep", dims, "cuda")
     with pytest.raises(ValueError):
         head.encode_context(torch.zeros(1, 3, 64), 2, 2, prefix=torch.zeros(2, 64))
+    with pytest.raises(ValueError):
+        _small_head("HipLlamaStep", _small_dims(), "cuda").encode_context(torch.zeros(1, 3, 64), 2, 2, prefix=torch.zeros(1, 2, 64))
     with pytest.raises(ValueError):
         head.train_logits(torch.zeros(1, 3, 64, device="cuda"), torch.zeros(1, 2, dtype=torch.long))
