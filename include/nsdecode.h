@@ -397,7 +397,10 @@ int nsd_swiglu(const void *gate_up, int64_t rows, int32_t inter, int32_t dtype, 
 /* ---- attention of whole sequences, and of a beam over long shared prefixes ------------------------------------
  * Shape of a call.  Query head hq reads kv head hq / (heads / kv_heads).  Strides count elements, in the order
  * (batch, position, head); the hd elements of a row are consecutive.  Pointers and strides must be multiples of 16
- * bytes, else NSD_E_ALIGN.  hd: a multiple of 8, 8 to 128; scale > 0; dtype 0 = fp32, 1 = bf16. */
+ * bytes, else NSD_E_ALIGN.  hd: a multiple of 8, 8 to 128; scale > 0; dtype 0 = fp32, 1 = bf16.  len_k and
+ * len_q * heads / kv_heads at most 2^30; a launch has fewer than 2^24 workgroups: batch * kv_heads times
+ * len_q * heads / kv_heads / 128 (/ 64 or / 32 where that is one tile), and times len_k / 64 (/ 32) for the gradients;
+ * else NSD_E_SIZE. */
 typedef struct NsdSeqAttn {
     int32_t batch, len_q, len_k, heads, kv_heads, hd, dtype;
     int32_t causal;                    /* query i sees keys j <= i + len_k - len_q (none for the first rows if len_q > len_k) */

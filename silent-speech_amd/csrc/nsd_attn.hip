@@ -128,19 +128,23 @@ nsd_add_rmsnorm_row_kernel(const T *x, const T *delta, const T *w, float eps, in
     }
 }
 
+constexpr int64_t MAX_THREADS = 4294967295ll;                   // a launch counts its threads in 32 bits
+
 template <class T>
-void launch_add_rmsnorm(const T *x, const T *delta, const T *w, float eps, int rows, int hidden, T *x_out, T *h, hipStream_t s)
+int launch_add_rmsnorm(const T *x, const T *delta, const T *w, float eps, int rows, int hidden, T *x_out, T *h, hipStream_t s)
 {
     // two 16-byte pieces per lane (one or four measure the same or worse at 1 024 x 3 072 bf16: 8.1 / 8.0 / 8.8 us)
     constexpr int VN = Vec16<T>::N, NV = 2;
     const int nvec = hidden / VN;
     const int waves = (nvec + 64 * NV - 1) / (64 * NV);
+    if (rows > MAX_THREADS / (waves <= 16 ? 64 * waves : 64) - 3) return NSD_E_SIZE;
     if (waves <= 16)
         hipLaunchKernelGGL((nsd_add_rmsnorm_row_kernel<T, NV>), dim3((unsigned)rows), dim3(64 * waves), 0, s,
                            x, delta, w, eps, hidden, x_out, h);
     else
         hipLaunchKernelGGL(nsd_add_rmsnorm_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s,
                            x, delta, w, eps, rows, hidden, x_out, h);
+    return (int)hipGetLastError();
 }
 
 // ---------------------------------------------------------------------
@@ -337,6 +341,8 @@ int launch_add_rmsnorm_bwd(const T *x, const T *w, const T *dh, const T *dx_out,
 {
     constexpr int VN = Vec16<T>::N, NV = 2;
     const int nvec = hidden / VN, waves = (nvec + 64 * NV - 1) / (64 * NV), parts = norm_bwd_parts(rows, hidden);
+    // (rows: the walk's index plus its step stays in 31 bits; hidden: the 16 threads a column of the column sums)
+    if (rows > (1 << 30) || (waves > 16 && rows > MAX_THREADS / 1024) || (dw && hidden >= 1 << 28)) return NSD_E_SIZE;
     if (waves <= 16) {
         hipLaunchKernelGGL((nsd_add_rmsnorm_bwd_kernel<T, NV>), dim3((unsigned)parts), dim3(64 * waves), 0, s,
                            x, w, dh, dx_out, eps, rows, hidden, dx, dw ? ws : nullptr);
@@ -559,7 +565,7 @@ nsd_attn_step_kernel(AttnArgs a)
                 vr = vctx + (size_t)p * hd;
             } else {
                 const int s = p - S;
-                const int slot = s == t ? m : u * a.B + (int)a.anc[(size_t)s * M + m];
+                const int slot = s == t ? m : u * a.B + min((int)a.anc[(size_t)s * M + m], a.B - 1);
                 const size_t off = (((size_t)s * M + slot) * a.kvh + h) * hd;
                 kr = kgen + off;
                 vr = vgen + off;
@@ -790,7 +796,7 @@ int launch_attn_g(const AttnArgs &a, hipStream_t s)
     const size_t per_wave = q_bytes + (size_t)G * 64 * 4 + 64 * 8;
     int waves = a.B < 16 ? a.B : 16;
     while (waves > 1 && per_wave * waves > 65536) --waves;
-    if (per_wave > 65536) return NSD_E_SIZE;
+    if (per_wave > 65536 || (int64_t)a.N * a.kvh > MAX_THREADS / (64 * waves)) return NSD_E_SIZE;
     const dim3 grid((unsigned)(a.N * a.kvh), (unsigned)((a.B + waves - 1) / waves));
     hipLaunchKernelGGL((nsd_attn_step_kernel<T, G>), grid, dim3(64 * waves), per_wave * waves, s, a);
     return (int)hipGetLastError();
@@ -834,12 +840,10 @@ extern "C" int nsd_add_rmsnorm(const void *x, const void *delta, const void *w, 
     if (!x || !w || !h || (delta && !x_out)) return NSD_E_NULL;
     if (!aligned16(x, delta, w, x_out, h)) return NSD_E_ALIGN;
     if (dtype == 0)
-        launch_add_rmsnorm<float>((const float *)x, (const float *)delta, (const float *)w, eps, rows, hidden,
-                                  (float *)x_out, (float *)h, (hipStream_t)stream);
-    else
-        launch_add_rmsnorm<BF16>((const BF16 *)x, (const BF16 *)delta, (const BF16 *)w, eps, rows, hidden,
-                                 (BF16 *)x_out, (BF16 *)h, (hipStream_t)stream);
-    return (int)hipGetLastError();
+        return launch_add_rmsnorm<float>((const float *)x, (const float *)delta, (const float *)w, eps, rows, hidden,
+                                         (float *)x_out, (float *)h, (hipStream_t)stream);
+    return launch_add_rmsnorm<BF16>((const BF16 *)x, (const BF16 *)delta, (const BF16 *)w, eps, rows, hidden,
+                                    (BF16 *)x_out, (BF16 *)h, (hipStream_t)stream);
 }
 
 extern "C" int64_t nsd_add_rmsnorm_bwd_workspace(int32_t rows, int32_t hidden)
@@ -857,6 +861,7 @@ extern "C" int nsd_add_rmsnorm_bwd(const void *x_out, const void *w, const void 
     if (!aligned16(x_out, w, dh, dx_out, dx, dw, ws)) return NSD_E_ALIGN;
     if (dw && ws_bytes < nsd_add_rmsnorm_bwd_workspace(rows, hidden)) return NSD_E_SIZE;
     if (rows == 0) {                                            // a sum over no rows
+        if (hidden >= 1 << 28) return NSD_E_SIZE;
         const dim3 grid((unsigned)((hidden + 63) / 64)), block(1024);
         if (dtype == 0) hipLaunchKernelGGL(nsd_colsum_kernel<float>, grid, block, 0, (hipStream_t)stream, nullptr, 0, hidden, (float *)dw);
         else hipLaunchKernelGGL(nsd_colsum_kernel<BF16>, grid, block, 0, (hipStream_t)stream, nullptr, 0, hidden, (BF16 *)dw);

@@ -1079,6 +1079,7 @@ nsd_attn_bwd_kv_kernel(SeqArgs a)
 // launchers
 // ---------------------------------------------------------------------
 constexpr int CUS = 256;
+constexpr int64_t MAX_WGS = (1 << 24) - 1;                      // of 256 threads: a launch counts its threads in 32 bits
 
 struct Plan { int wave_rows, bn, tiles, splits, split_tiles; };
 
@@ -1236,7 +1237,15 @@ int shape_check(const NsdSeqAttn *p)
     if (R > (1ll << 30) || R * G >= (1ll << 32) || p->len_k > (1 << 30)) return NSD_E_SIZE;
     const int64_t zk = (int64_t)p->batch * p->kv_heads;
     if (zk > (1ll << 30) || zk * ((R + 31) / 32) > (1ll << 30) || zk * (((int64_t)p->len_k + 31) / 32) > (1ll << 30)) return NSD_E_SIZE;
+    if (zk * div_up(R, R <= 32 ? 32 : R <= 64 ? 64 : 128) > MAX_WGS) return NSD_E_SIZE;    // (the tiles of many rows)
     return NSD_OK;
+}
+
+int bwd_shape_check(const NsdSeqAttn *p)
+{
+    if (const int rc = shape_check(p)) return rc;
+    if (p->key_len) return NSD_E_SIZE;                          // ragged keys are a form of the prefix state only
+    return (int64_t)p->batch * p->kv_heads * div_up(p->len_k, p->len_k <= 32 ? 32 : 64) > MAX_WGS ? NSD_E_SIZE : NSD_OK;
 }
 
 // the same as kernel arguments, with the pointers and strides checked (in pieces of 16 bytes)
@@ -1305,7 +1314,7 @@ extern "C" int nsd_attn_fwd(const void *q, const void *k, const void *v, const N
 
 extern "C" int64_t nsd_attn_bwd_workspace(const NsdSeqAttn *p)
 {
-    if (shape_check(p) || p->batch == 0) return 0;
+    if (bwd_shape_check(p) || p->batch == 0) return 0;
     const int R = p->len_q * (p->heads / p->kv_heads);
     const BwdScratch b = bwd_scratch(bwd_q_plan(p->batch, p->kv_heads, R, p->len_k, p->hd, p->dtype),
                                      bwd_kv_plan(p->batch, p->kv_heads, R, p->len_k, p->hd, p->dtype),
@@ -1318,8 +1327,8 @@ extern "C" int nsd_attn_bwd(const void *q, const void *k, const void *v, const v
                             void *stream)
 {
     SeqArgs a;
+    if (const int rc = bwd_shape_check(p)) return rc;
     if (const int rc = seq_args(p, q, k, v, a)) return rc;
-    if (p->key_len) return NSD_E_SIZE;                          // ragged keys are a form of the prefix state only
     if (p->batch == 0) return NSD_OK;
     if (a.R > 0 && (!out || !lse || !dout || !dq || !ws)) return NSD_E_NULL;
     if (a.Lk > 0 && (!dk || !dv)) return NSD_E_NULL;

@@ -479,6 +479,42 @@ def test_c_entries_refuse_what_they_cannot_do():
     assert nb(n=4) == SIZE and nb(x=A + 2) == lib.E_ALIGN and nb(rows=0, dw=None) == 0
 
 
+def test_c_entries_refuse_launches_of_2_to_the_32_threads():
+    lib, L = _lib()
+    A, SIZE, many = 4096, -7, 1 << 24
+    one = dict(heads=1, kv_heads=1, hd=8, len_q=1, len_k=1, causal=0)
+    for p in (_seq(**{**one, "batch": many}), _seq(**{**one, "batch": many // 64, "len_q": 8192}),
+              _seq(**{**one, "batch": many // 4, "kv_heads": 4, "heads": 4})):
+        assert L.nsd_attn_fwd(A, A, A, C.byref(p), A, None, None, None, 0, None) == SIZE
+        assert L.nsd_attn_prefix(A, A, A, C.byref(p), 0, A, A, A, None, 0, None) == SIZE
+        assert L.nsd_attn_bwd(A, A, A, A, A, None, A, C.byref(p), A, A, A, A, 1 << 62, None) == SIZE
+    p = _seq(**{**one, "batch": many // 2, "len_k": 65})          # two tiles of keys for each sequence
+    assert L.nsd_attn_fwd_workspace(C.byref(p)) == 0 and L.nsd_attn_bwd_workspace(C.byref(p)) == 0
+    assert L.nsd_attn_bwd(A, A, A, A, A, None, A, C.byref(p), A, A, A, A, 1 << 62, None) == SIZE
+    p = _seq(**{**one, "batch": many // 2, "len_k": 64})
+    assert L.nsd_attn_bwd_workspace(C.byref(p)) > 0
+    norm = lambda rows, hidden: L.nsd_add_rmsnorm(A, None, A, 1e-5, rows, hidden, 1, None, A, None)   # noqa: E731
+    assert norm(1 << 26, 8) == SIZE and norm(1 << 24, 4096) == SIZE and norm((1 << 31) - 1, 1 << 20) == SIZE
+    back = lambda rows, hidden: L.nsd_add_rmsnorm_bwd(A, A, A, None, 1e-5, rows, hidden, 1, A, A, A, 1 << 62, None)   # noqa: E731
+    assert back((1 << 31) - 1, 8) == SIZE and back(1 << 22, 1 << 15) == SIZE and back(0, 1 << 28) == SIZE and back(4, 1 << 28) == SIZE
+    step = lambda N, B, kvh: L.nsd_attn_step(A, None, None, A, A, A, A, N, B, kvh, kvh, 8, 0, 1, 0.3, 1, None, None, None, None)   # noqa: E731
+    assert step(1 << 26, 1, 1) == SIZE and step(1 << 20, 16, 4) == SIZE and step(1 << 30, 1, 1 << 10) == SIZE
+
+
+@pytest.mark.gpu
+def test_beam_step_holds_its_ancestors_to_the_beam():
+    """A table entry past the beam reads the beam's last slot."""
+    from silent_speech_amd import ops
+    g = _gen(11)
+    N, B, t, D = 3, 4, 5, 64
+    kg, vg = (torch.randn(t + 1, N * B, 2, D, generator=g).to(BF).cuda() for _ in range(2))
+    q = torch.randn(N * B, 4, D, generator=g).to(BF).cuda()
+    anc = torch.randint(0, 256, (t, N * B), generator=g).to(torch.uint8)
+    a = ops.shared_prefix_attention(q, [], kg, vg, anc.cuda(), t, B)
+    b = ops.shared_prefix_attention(q, [], kg, vg, anc.clamp(max=B - 1).cuda(), t, B)
+    assert torch.equal(a, b)
+
+
 def test_python_entries_refuse_what_they_cannot_do():
     from silent_speech_amd import lib, ops
     z = lambda *s, dt=BF: torch.zeros(*s, dtype=dt)             # noqa: E731
