@@ -1086,7 +1086,7 @@ struct Plan { int wave_rows, bn, tiles, splits, split_tiles; };
 int dp_of(int D) { return D <= 64 ? 64 : 128; }
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How often the walk over `steps` tiles is split so that `room` workgroups are on the card: whole shares, as a few more
+// Backward: how often the walk over `steps` tiles is split so that `room` workgroups are on the card: whole shares, as a few more
 // workgroups than there is room for cost a second round; no share shorter than `least`, below which the join costs more
 // than the split gives.
 void split_walk(Plan &p, int64_t wgs, int64_t steps, int64_t room, int64_t least)
@@ -1095,6 +1095,28 @@ void split_walk(Plan &p, int64_t wgs, int64_t steps, int64_t room, int64_t least
     s = s > steps / least ? steps / least : s;
     p.split_tiles = (int)(s > 1 ? div_up(steps, s) : steps > 0 ? steps : 1);
     p.splits = (int)(s > 1 ? div_up(steps, p.split_tiles) : 1);
+}
+
+// Forward: the split with the least of (tiles of a share) x (time of a tile) + (time of the join).  In ns, with keys that
+// come from memory as a decode's do (another layer's lie between two steps): a bf16 tile takes 1330 and 1950 (head
+// dimensions up to 64 and 128; 1600 with few rows) whether one workgroup waits for it on a CU or two, an fp32 tile 3100
+// and 5200, with two workgroups 1.5 and 2 times that; the join takes 3 us and 33 ns for each share of 128 rows.  A beam step
+// over one prefix, 8 kv heads, as many workgroups as there is room for against this: 1024 hypotheses, 24 heads of 128: 512
+// positions 54 and 44 us, 2048 77 and 77, 8192 170 and 170 (2048 without a split: 91); 512 with 16 heads of 64: 26 and 25,
+// 41 and 36, 56 and 56.
+void split_keys(Plan &p, int64_t wgs, int64_t steps, int DP, int dtype)
+{
+    const bool wide = DP == 128;
+    const int64_t tile = dtype == 0 ? (wide ? 5200 : 3100) : p.wave_rows < 4 ? 1600 : wide ? 1950 : 1330;
+    const int64_t pair = dtype == 0 ? (wide ? 200 : 150) : 100;  // percent
+    int64_t best = 1, least = steps * tile;
+    for (int64_t s = 2; s <= steps && s * wgs <= 2 * CUS; ++s) {
+        const int64_t share = div_up(steps, s);
+        const int64_t t = share * tile * (s * wgs > CUS ? pair : 100) / 100 + 3000 + s * wgs * p.wave_rows * 33 / 4;
+        if (t < least) { least = t; best = s; }
+    }
+    p.split_tiles = (int)(best > 1 ? div_up(steps, best) : steps > 0 ? steps : 1);
+    p.splits = (int)(best > 1 ? div_up(steps, p.split_tiles) : 1);
 }
 
 // Forward: row tiles of 128 (four waves along the rows) unless there are at most 64 or 32 rows: the waves then share the
@@ -1107,7 +1129,7 @@ Plan fwd_plan(int Z, int KVH, int R, int Lk, int D, int dtype)
     p.wave_rows = R <= 32 ? 1 : R <= 64 ? 2 : 4;
     p.bn = (dtype == 0 || p.wave_rows < 4 ? 32 : 64) * (4 / p.wave_rows);
     p.tiles = (int)div_up(R, 32 * p.wave_rows);
-    split_walk(p, (int64_t)p.tiles * KVH * Z, div_up(Lk, p.bn), 2 * CUS, dtype == 0 ? 1 : 4);
+    split_keys(p, (int64_t)p.tiles * KVH * Z, div_up(Lk, p.bn), dp_of(D), dtype);
     return p;
 }
 
