@@ -149,8 +149,9 @@ int launch_add_rmsnorm(const T *x, const T *delta, const T *w, float eps, int ro
 
 // ---------------------------------------------------------------------
 // backward of residual add + RMSNorm.  With r = rsqrt(mean(x^2) + eps), xh = x r and g = dh w:
-//   dx = dx_out + r (g - xh mean(g xh)) = dx_out + r g - x r^3 mean(g x),   dw = sum over the rows of dh xh.
-// Both row sums are taken in one pass.  A workgroup holds a row in registers as the forward does, and walks over rows
+//   dx = dx_out + r (g - xh mean(g xh)),   mean(g xh) = r mean(g x),   dw = sum over the rows of dh xh.
+// Both row sums are taken in one pass.  The factors stay apart as they stand there: a power of r of its own leaves fp32
+// where the rows' squares do not (r^3 for rows of 1e13 and more, or of 1e-13 and less).  A workgroup holds a row in registers as the forward does, and walks over rows
 // blockIdx.x, + gridDim.x, ...: a thread then meets the same columns in every row and keeps their part of dw in
 // registers; the workgroups' parts (fp32) are summed in a fixed order by nsd_colsum_kernel.
 // ---------------------------------------------------------------------
@@ -199,15 +200,16 @@ nsd_add_rmsnorm_bwd_kernel(const T *x, const T *w, const T *dh, const T *dx_out,
         ss = gx = 0.0f;
         for (int q = 0; q < waves; ++q) { ss += part[buf][0][q]; gx += part[buf][1][q]; }
         const float r = rsqrtf(ss / (float)hidden + eps);
-        const float c = r * r * r * (gx / (float)hidden);
+        const float m = r * (gx / (float)hidden);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int i = (int)threadIdx.x + k * (int)blockDim.x;
             if (i < nvec) {
 #pragma unroll
                 for (int e = 0; e < VN; ++e) {
-                    dw[k][e] = __builtin_fmaf(gv[k][e], xv[k][e] * r, dw[k][e]);
-                    const float d = __builtin_fmaf(gv[k][e] * wv[k][e], r, -(xv[k][e] * c));
+                    const float xh = xv[k][e] * r;
+                    dw[k][e] = __builtin_fmaf(gv[k][e], xh, dw[k][e]);
+                    const float d = r * __builtin_fmaf(-xh, m, gv[k][e] * wv[k][e]);
                     xv[k][e] = dx_out ? ov[k][e] + d : d;
                 }
                 Store16<T>::store(dx + base + (size_t)i * VN, xv[k]);
@@ -258,7 +260,7 @@ nsd_add_rmsnorm_bwd_long_kernel(const T *x, const T *w, const T *dh, const T *dx
     ss = gx = 0.0f;
     for (int q = 0; q < (int)(blockDim.x >> 6); ++q) { ss += part[0][q]; gx += part[1][q]; }
     const float r = rsqrtf(ss / (float)hidden + eps);
-    const float c = r * r * r * (gx / (float)hidden);
+    const float m = r * (gx / (float)hidden);
     for (int i = (int)threadIdx.x * VN; i < hidden; i += (int)blockDim.x * VN) {
         float xv[8], gv[8], wv[8], ov[8];
         Vec16<T>::load(x + base + i, xv);
@@ -267,7 +269,7 @@ nsd_add_rmsnorm_bwd_long_kernel(const T *x, const T *w, const T *dh, const T *dx
         if (dx_out) Vec16<T>::load(dx_out + base + i, ov);
 #pragma unroll
         for (int e = 0; e < VN; ++e) {
-            const float d = __builtin_fmaf(gv[e] * wv[e], r, -(xv[e] * c));
+            const float d = r * __builtin_fmaf(-(xv[e] * r), m, gv[e] * wv[e]);
             xv[e] = dx_out ? ov[e] + d : d;
         }
         Store16<T>::store(dx + base + i, xv);
