@@ -62,6 +62,13 @@ int same_type(const char *name, const Tensor &first, std::initializer_list<const
             throw pybind11::type_error(std::string(name) + ": tensors of different types");
     return first.scalar_type() == at::kBFloat16;
 }
+// Tangents of forward-mode differentiation would be lost in the calls below, whether or not the tensor also requires a
+// gradient.
+void no_tangents(const char *name, std::initializer_list<const Tensor *> ts)
+{
+    for (const Tensor *t : ts)
+        if (t->defined() && t->_fw_grad(/*level=*/0).defined()) bad_value(std::string(name) + " has no forward-mode derivative");
+}
 double scale_or_default(const char *name, std::optional<double> scale, int64_t hd)
 {
     const double s = scale ? *scale : 1.0 / std::sqrt((double)hd);
@@ -156,6 +163,7 @@ struct Attention : torch::autograd::Function<Attention> {
     {
         const auto saved = ctx->get_saved_variables();
         const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &mask = saved[3], &out = saved[4], &lse = saved[5], &rest = saved[6];
+        no_tangents("attention's gradient", {&q, &k, &v, &grads[0]});
         variable_list d(6);
         {
             const c10::DeviceGuard guard(q.device());
@@ -186,6 +194,7 @@ Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v, bool causal,
     for (int64_t n : {Z, q.size(1), k.size(1), H})
         if (n > INT32_MAX) bad_value("attention: an axis of more than 2^31 - 1");
     Tensor mask = key_mask ? *key_mask : Tensor();
+    no_tangents("attention", {&q, &k, &v});
     same_device("attention", q, {&k, &v, &mask});
     same_type("attention", q, {&k, &v});
     if (mask.defined()) {
@@ -216,6 +225,9 @@ Tensor shared_prefix_attention(const Tensor &q0, const std::vector<std::vector<T
     if (D < 8 || D > 128 || (D & (D - 1))) bad_value(at_ + "head dimension " + std::to_string(D) + " is not a power of two from 8 to 128");
     if (beam < 1 || beam > NSD_MAX_BEAM || M % beam || t < 0 || t >= T || M > INT32_MAX)
         bad_value(at_ + "beam divides M and is at most 64, and 0 <= t < len(kgen)");
+    no_tangents(name, {&q0, &kgen, &vgen});
+    for (const auto &p : prefixes)
+        if (p.size() >= 2) no_tangents(name, {&p[0], &p[1]});
     same_device(name, q0, {&kgen, &vgen, &anc});
     const int dt = same_type(name, q0, {&kgen, &vgen});
     bool grad = q0.requires_grad() || kgen.requires_grad() || vgen.requires_grad();
@@ -304,6 +316,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
     {
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1];
+        no_tangents("add_rms_norm's gradient", {&x, &w, &grads[0], &grads[1]});
         const bool delta = ctx->saved_data["delta"].toBool();
         const bool want_w = ctx->needs_input_grad(delta ? 2 : 1);   // (counts the tensors among the inputs)
         variable_list d(4);
@@ -338,6 +351,7 @@ std::pair<Tensor, Tensor> add_rms_norm(const Tensor &x, const OptTensor &delta0,
     const Tensor delta = delta0 ? *delta0 : Tensor();
     if (x.dim() < 1 || w.dim() != 1 || w.size(0) != x.size(-1) || (delta.defined() && !delta.sizes().equals(x.sizes())))
         bad_value("add_rms_norm takes x and delta [..., hidden] and w [hidden]");
+    no_tangents("add_rms_norm", {&x, &delta, &w});
     same_device("add_rms_norm", x, {&delta, &w});
     const int dt = same_type("add_rms_norm", x, {&delta, &w}), unit = dt ? 8 : 4;
     const int64_t hidden = x.size(-1);

@@ -8,7 +8,7 @@ for prompts and scored candidates, and for beam steps over long prefixes.
 Device tensors in float32 or bfloat16; there is no CPU fall-back.  Kernels run on the current stream of the tensors'
 device; scratch comes from torch's allocator, call by call.  Same arguments, same bits.  Arguments are checked and the
 autograd nodes live in csrc/nsd_torch.cpp: ValueError and TypeError for arguments, NsdError for what the library
-refuses.
+refuses.  Derivatives are reverse-mode only: a tensor with a forward-mode tangent (torch.autograd.forward_ad) is refused.
 """
 from __future__ import annotations
 

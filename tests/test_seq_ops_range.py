@@ -26,3 +26,63 @@ def test_norm_gradients_of_large_and_small_rows(dtype, rows, hidden, size, eps):
     dx, dw = torch.autograd.grad(h, (xd, wd), dh.cuda())
     R.within(dx, want["dx"], "dx")
     R.within(dw, want["dw"], "dw")
+
+
+# ---------------------------------------------------------------------- derivatives that there are not
+def _dual_calls(dev, grad):
+    """(name, call with its arguments of which one is a dual tensor)"""
+    from silent_speech_amd import ops
+    z = lambda *s: torch.ones(*s, device=dev)                   # noqa: E731
+    dual = lambda x: torch.autograd.forward_ad.make_dual(x.requires_grad_(grad), torch.ones_like(x))   # noqa: E731
+    calls = []
+    for i in range(3):
+        def attention(i=i):
+            a = [z(1, 4, h, 16) for h in (4, 2, 2)]
+            a[i] = dual(a[i])
+            return ops.attention(*a)
+        def norm(i=i):                                           # noqa: E306
+            a = [z(3, 16), z(3, 16), z(16)]
+            a[i] = dual(a[i])
+            return ops.add_rms_norm(*a)
+        calls += [(f"attention {i}", attention), (f"add_rms_norm {i}", norm)]
+    for i in range(5):
+        def beam(i=i):
+            a = [z(4, 4, 16), z(1, 2, 5, 16), z(1, 2, 5, 16), z(1, 4, 2, 16), z(1, 4, 2, 16)]
+            a[i] = dual(a[i])
+            with torch.no_grad():
+                return ops.shared_prefix_attention(a[0], [(a[1], a[2])], a[3], a[4], None, 0, 2)
+        calls.append((f"shared_prefix_attention {i}", beam))
+    return calls
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    with torch.autograd.forward_ad.dual_level():
+        for name, call in _dual_calls("cpu", grad):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused_on_the_device(grad):
+    from silent_speech_amd import ops
+    with torch.autograd.forward_ad.dual_level():
+        for name, call in _dual_calls("cuda", grad):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        # a backward pass of a dual gradient: a derivative of the gradient
+        q, k = (torch.randn(1, 4, 2, 16, device="cuda").requires_grad_() for _ in range(2))
+        out = ops.attention(q, k, k)
+        with pytest.raises((ValueError, RuntimeError), match="forward-mode"):
+            torch.autograd.grad(out, q, torch.autograd.forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
+        x, w = torch.randn(3, 32, device="cuda").requires_grad_(), torch.ones(32, device="cuda")
+        y = ops.add_rms_norm(x, None, w)
+        for dual in range(2):
+            one = torch.ones_like(x)
+            go = [one, one]
+            go[dual] = torch.autograd.forward_ad.make_dual(one, torch.ones_like(one))
+            with pytest.raises((ValueError, RuntimeError), match="forward-mode"):
+                torch.autograd.grad(y, x, go, retain_graph=True)
+    q = torch.randn(1, 4, 2, 16, device="cuda")                 # outside of a level nothing is dual
+    assert ops.attention(q, q, q).shape == q.shape
