@@ -429,7 +429,7 @@ int nsd_attn_fwd(const void *q, const void *k, const void *v, const NsdSeqAttn *
 /* Gradients of that attention for dout [batch, len_q, heads, hd]; out, lse and rest (or NULL) as nsd_attn_fwd left
  * them.
  *   dq [batch, len_q, heads, hd], dk, dv [batch, len_k, kv_heads, hd] (summed over the query heads of a kv head);
- *   zeros for masked keys and for rows that see no key.  ws: nsd_attn_bwd_workspace(p) bytes. */
+ *   zeros for masked keys and for rows that see no key, whatever q and dout hold there.  ws: nsd_attn_bwd_workspace(p) bytes. */
 int64_t nsd_attn_bwd_workspace(const NsdSeqAttn *p);
 int nsd_attn_bwd(const void *q, const void *k, const void *v, const void *out, const float *lse, const uint8_t *rest,
                  const void *dout, const NsdSeqAttn *p, void *dq, void *dk, void *dv, void *ws, int64_t ws_bytes, void *stream);

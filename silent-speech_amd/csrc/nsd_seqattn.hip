@@ -905,6 +905,7 @@ nsd_attn_bwd_kv_kernel(SeqArgs a)
     static_assert(WR == 1 || 2 * NBUF * TB >= 4 * 32 * DP * 4, "the waves' sums meet in the tiles' place");
     __shared__ __align__(16) char smem[2 * NBUF * TB];
     __shared__ __align__(16) float stat[NBUF][2][BM];
+    __shared__ int unseen[NBUF][BM / 64];                       // whether a tile has rows that saw no key, of 64 each
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c32 = lane & 31;
     const int wk = w % WK, wr = w / WK;
     int pair, kt;                                               // the first keys are seen by most rows
@@ -966,7 +967,18 @@ nsd_attn_bwd_kv_kernel(SeqArgs a)
         if (threadIdx.x < BM) {
             stat[b][0][threadIdx.x] = st_l;
             stat[b][1][threadIdx.x] = st_d;
+            unseen[b][threadIdx.x >> 6] = __ballot(st_l == -__builtin_inff()) != 0;
         }
+    };
+    // A row that saw no key has part in nothing, so what its query and its gradient hold (the padding in front of a
+    // sequence) may be NaN, which 0 * NaN would spread over dK and dV: zeros instead.  (In the tile, once it is there: left
+    // out while it is fetched, by the log-sums of a tile before, the kernel spills and the tiles wait for those.  The question
+    // takes 1 of 88 us at 8 x 640 positions.)
+    auto blank = [&](int b, char *sq, char *sg) {
+        for (int i = threadIdx.x; i < TB / 16; i += 256)
+            if (stat[b][0][i / 64 / TL::CG * 16 + (i & 63) / 4] == -__builtin_inff())
+                *reinterpret_cast<uint4 *>(sq + i * 16) = *reinterpret_cast<uint4 *>(sg + i * 16) = make_uint4(0, 0, 0, 0);
+        __syncthreads();
     };
     if (NBUF == 2 && t >= t_first) {
         fetch(t, smem);
@@ -981,6 +993,12 @@ nsd_attn_bwd_kv_kernel(SeqArgs a)
         }
         tile_barrier();
         if (NBUF == 2 && t > t_first) fetch(t - 1, smem + (buf ^ 1) * 2 * TB);
+        if (a.mask || off < 0) {                                // (else every row sees a key)
+            int none = 0;
+#pragma unroll
+            for (int i = 0; i < BM / 64; ++i) none |= unseen[buf][i];
+            if (__builtin_amdgcn_readfirstlane(none)) blank(buf, sq, sg);
+        }
 #pragma unroll 1
         for (int i = 0; i < NS; ++i) {
             const int n = wr + WR * i;

@@ -51,7 +51,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     q [Z, Lq, heads, hd]; k, v [Z, Lk, kv_heads, hd], heads a multiple of kv_heads (query head i reads kv head
     i // (heads // kv_heads)); hd a multiple of 8 up to 128; any strides.  causal: query i sees keys j <= i + Lk - Lq.
     key_mask [Z, Lk] bool (or uint8): keys that are False are seen by no query, whatever they hold.  A query that sees
-    no key gives zeros, and no gradient.  scale > 0, default 1 / sqrt(hd).  Returns [Z, Lq, heads, hd]."""
+    no key gives zeros and has no part in any gradient, whatever it and its row of the output's gradient hold.  scale > 0,
+    default 1 / sqrt(hd).  Returns [Z, Lq, heads, hd]."""
     return (_torch_side or load()).attention(q, k, v, causal, key_mask, scale)
 
 

@@ -1,4 +1,6 @@
 """The sequence operators over the range that they are documented for."""
+import math
+
 import pytest
 import torch
 
@@ -86,3 +88,39 @@ def test_forward_mode_is_refused_on_the_device(grad):
                 torch.autograd.grad(y, x, go, retain_graph=True)
     q = torch.randn(1, 4, 2, 16, device="cuda")                 # outside of a level nothing is dual
     assert ops.attention(q, q, q).shape == q.shape
+
+
+# ---------------------------------------------------------------------- rows that see no key
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("Z,L,KVH,G,D,pad", [
+    (2, 50, 1, 2, 64, "left"), (2, 150, 2, 3, 128, "left"), (16, 67, 8, 2, 64, "left"), (16, 67, 8, 2, 128, "left"),
+    (32, 23, 8, 2, 128, "left"), (2, 90, 1, 2, 64, "short"), (3, 40, 2, 1, 128, "none"), (1, 600, 1, 8, 64, "left")])
+def test_what_rows_without_keys_hold_takes_no_part(dtype, Z, L, KVH, G, D, pad):
+    """A batch padded on the left whose padding holds NaN everywhere (or fewer keys than queries under a causal mask, or a
+    sequence that sees nothing): such a row gives zeros and has no part in any gradient, whatever its query and its
+    gradient hold."""
+    from silent_speech_amd import ops
+    g = _gen(L + D)
+    Lk = L // 2 if pad == "short" else L
+    q, k, v = (torch.randn(Z, n, h, D, generator=g).to(dtype) for n, h in ((L, KVH * G), (Lk, KVH), (Lk, KVH)))
+    do = torch.randn(Z, L, KVH * G, D, generator=g).to(dtype)
+    mask = torch.ones(Z, Lk, dtype=torch.bool)
+    rows = torch.zeros(Z, L, dtype=torch.bool)                  # that see no key
+    if pad == "short":
+        rows[:, :L - Lk] = True
+    for z in range(Z):
+        n = (5 * z + 3) % L if pad == "left" else L if pad == "none" and z == 1 else 0
+        if n:
+            mask[z, :n] = False
+            rows[z, :n] = True
+    at = rows[:, :, None, None]
+    want = R.attention(q.masked_fill(at, 0.0), k, v, True, mask, 1 / math.sqrt(D), do.masked_fill(at, 0.0))
+    k, v = (x.masked_fill(~mask[:, :, None, None], float("nan")) for x in (k, v))
+    leaves = [x.cuda().requires_grad_() for x in (q.masked_fill(at, float("nan")), k, v)]
+    out = ops.attention(*leaves, key_mask=None if pad == "short" else mask.cuda())
+    R.within(out, want["out"], "out")
+    grads = torch.autograd.grad(out, leaves, do.masked_fill(at, float("inf")).cuda())
+    for name, x in zip(("dq", "dk", "dv"), grads):
+        R.within(x, want[name], name)
+    assert not bool(grads[0][rows.cuda()].any())
