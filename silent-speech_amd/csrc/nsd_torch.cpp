@@ -195,6 +195,12 @@ Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v, bool causal,
         if (n > INT32_MAX) bad_value("attention: an axis of more than 2^31 - 1");
     Tensor mask = key_mask ? *key_mask : Tensor();
     no_tangents("attention", {&q, &k, &v});
+    const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+    if (grad && Z > 0) {                                        // a shape that only the gradients refuse is refused here
+        NsdSeqAttn p = seq_of(q, k, v, Tensor(), causal, 1.0);
+        p.len_q = p.len_q > 0 ? p.len_q : 1;                    // (no queries need no scratch either)
+        if (!lib.attn_bwd_workspace(&p)) check(NSD_E_SIZE, "nsd_attn_bwd");
+    }
     same_device("attention", q, {&k, &v, &mask});
     same_type("attention", q, {&k, &v});
     if (mask.defined()) {
@@ -203,7 +209,7 @@ Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v, bool causal,
         mask = mask.contiguous();
     }
     const double s = scale_or_default("attention", scale, D);
-    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    if (grad)
         return Attention::apply(q, k, v, mask.defined() ? OptTensor(mask) : OptTensor(), causal, s);
     const at::AutoGradMode no_grad(false);
     return attn_fwd(in_rows(q), in_rows(k), in_rows(v), mask, causal, s, nullptr, nullptr);

@@ -90,6 +90,21 @@ def test_forward_mode_is_refused_on_the_device(grad):
     assert ops.attention(q, q, q).shape == q.shape
 
 
+# ---------------------------------------------------------------------- shapes that only the gradients refuse
+def test_attention_refuses_before_the_forward_pass_what_its_gradients_refuse():
+    from silent_speech_amd import lib, ops
+    one = lambda *s: torch.zeros(1, dtype=BF).expand(*s)       # noqa: E731
+    for lq in (1, 0):
+        q, k = one(1 << 23, lq, 1, 8), one(1 << 23, 65, 1, 8).requires_grad_()
+        with pytest.raises(lib.NsdError, match="nsd_attn_bwd"):
+            ops.attention(q, k, k.detach())
+        with pytest.raises(lib.NsdError, match="device"):       # without gradients the shape is fine
+            ops.attention(q, k.detach(), k.detach())
+    q, k = one(1 << 23, 1, 1, 8), one(1 << 23, 64, 1, 8).requires_grad_()
+    with pytest.raises(lib.NsdError, match="device"):
+        ops.attention(q, k, k.detach())
+
+
 # ---------------------------------------------------------------------- rows that see no key
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF, FP])
