@@ -368,7 +368,9 @@ __device__ const uint4 zero_page[1] = {};
 
 NSD_D void to_lds(uint64_t g, uint32_t lds)
 {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(g), "s"(lds) : "memory");
+    uint32_t m0;                                                // left as it was: the compiler may keep a value of its own there
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(g), "s"(lds) : "memory");
 }
 // every wave's loads have arrived, and every wave is done with what they will overwrite next
 NSD_D void tile_barrier()

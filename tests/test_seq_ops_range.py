@@ -1,5 +1,7 @@
 """The sequence operators over the range that they are documented for."""
 import math
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -139,3 +141,18 @@ def test_what_rows_without_keys_hold_takes_no_part(dtype, Z, L, KVH, G, D, pad):
     for name, x in zip(("dq", "dk", "dv"), grads):
         R.within(x, want[name], name)
     assert not bool(grads[0][rows.cuda()].any())
+
+
+# ---------------------------------------------------------------------- assembly leaves m0 alone
+def test_assembly_restores_m0():
+    """m0 is the compiler's (it keeps the index of a register array there, for instance, and cannot be told that a statement
+    overwrites it): a statement that needs it puts back what it found."""
+    seen = 0
+    for path in sorted((Path(__file__).parent.parent / "silent-speech_amd" / "csrc").iterdir()):
+        for text in re.findall(r'\basm volatile\(((?:\s*"[^"]*")+)', path.read_text()):
+            steps = [x.strip() for x in text.replace('"', "").replace("\\t", "").split("\\n")]
+            if any(re.match(r"s_mov_b32 m0,", x) for x in steps):
+                seen += 1
+                saved = re.fullmatch(r"s_mov_b32 (%\d), m0", steps[0])
+                assert saved and steps[-1] == f"s_mov_b32 m0, {saved[1]}", (path.name, text)
+    assert seen
