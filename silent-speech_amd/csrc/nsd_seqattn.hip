@@ -1154,7 +1154,8 @@ Plan fwd_plan(int Z, int KVH, int R, int Lk, int D, int dtype)
 }
 
 // Backward, dQ: 128 rows where that makes a workgroup for every CU, else 64 or 32 (the waves share the keys): fp32, 3 x 217
-// positions of 6 heads, 51 us with 128 rows, 27 with 32, 21 with the keys split as well.
+// positions of 6 heads, 51 us with 128 rows, 27 with 32, 21 with the keys split as well.  (tests/test_seq_ops_range.py restates
+// this choice and bwd_kv_plan's to reach every form.)
 Plan bwd_q_plan(int Z, int KVH, int R, int Lk, int D, int dtype)
 {
     Plan p;

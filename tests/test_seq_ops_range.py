@@ -7,9 +7,10 @@ import pytest
 import torch
 
 from tests import seq_reference as R
-from tests.test_seq_ops import _gen
+from tests.test_seq_ops import _gen, _mask
 
 BF, FP = torch.bfloat16, torch.float32
+CUS = 256
 
 
 # ---------------------------------------------------------------------- gradients of large and small rows of a norm
@@ -105,6 +106,46 @@ def test_attention_refuses_before_the_forward_pass_what_its_gradients_refuse():
     q, k = one(1 << 23, 1, 1, 8), one(1 << 23, 64, 1, 8).requires_grad_()
     with pytest.raises(lib.NsdError, match="device"):
         ops.attention(q, k, k.detach())
+
+
+# ---------------------------------------------------------------------- every form of the backward kernels
+def _plans(Z, KVH, R_, Lk):
+    """Waves along the rows (dQ) and along the keys (dK, dV) of a workgroup, as bwd_q_plan and bwd_kv_plan choose them (the
+    kernels' names in a trace of these shapes carry the same numbers)."""
+    pairs, up = Z * KVH, lambda a, b: -(-a // b)                # noqa: E731
+    q = 4 if R_ > 64 and pairs * up(R_, 128) >= CUS else 2 if R_ > 32 and pairs * up(R_, 64) >= CUS else 1
+    return q, 2 if Lk > 32 and pairs * up(Lk, 64) >= CUS // 2 else 1
+
+
+FORMS = [  # Z, Lq, Lk, kv heads, G, causal, mask, plans of dQ and of dK, dV
+    (16, 67, 67, 8, 2, True, None, (4, 2)), (16, 67, 150, 8, 2, True, "random", (4, 2)), (43, 45, 71, 3, 3, False, "pad", (4, 2)),
+    (16, 131, 67, 8, 1, True, "empty", (4, 2)), (86, 300, 300, 1, 1, True, "pad", (4, 2)), (32, 23, 45, 8, 2, True, "random", (2, 2)),
+    (32, 47, 33, 8, 1, True, None, (2, 2)), (43, 11, 129, 6, 5, False, "empty", (2, 2)), (32, 40, 31, 8, 1, False, "pad", (2, 1)),
+    # more pairs of an XCD than it works on together
+    (64, 70, 140, 8, 4, True, "pad", (4, 2)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (BF, 64), (BF, 72), (FP, 128), (FP, 64), (FP, 40)])
+@pytest.mark.parametrize("Z,Lq,Lk,KVH,G,causal,kind,plans", FORMS)
+def test_attention_gradients_in_every_form(dtype, D, Z, Lq, Lk, KVH, G, causal, kind, plans):
+    from silent_speech_amd import ops
+    assert _plans(Z, KVH, Lq * G, Lk) == plans
+    g = _gen(Lq + 3 * Lk + D)
+    q, k, v = (torch.randn(Z, n, h, D, generator=g).to(dtype) for n, h in ((Lq, KVH * G), (Lk, KVH), (Lk, KVH)))
+    do = torch.randn(Z, Lq, KVH * G, D, generator=g).to(dtype)
+    mask = _mask(kind, Z, Lk, g)
+    if mask is not None:
+        k = k.masked_fill(~mask[:, :, None, None], float("nan"))
+        v = v.masked_fill(~mask[:, :, None, None], float("inf"))
+    scale = 1.3 / math.sqrt(D)
+    want = R.attention(q, k, v, causal, mask, scale, do)
+    leaves = [x.cuda().requires_grad_() for x in (q, k, v)]
+    out = ops.attention(*leaves, causal=causal, key_mask=None if mask is None else mask.cuda(), scale=scale)
+    R.within(out, want["out"], "out")
+    for name, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, do.cuda())):
+        R.within(x, want[name], name)
 
 
 # ---------------------------------------------------------------------- rows that see no key
