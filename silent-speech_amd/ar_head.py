@@ -364,6 +364,7 @@ class HipLlamaStep(TorchLlamaStep):
     reads the context again for every hypothesis).  Both sum the same terms in another order."""
 
     _DT = {torch.float32: 0, torch.bfloat16: 1}
+    JOIN_BYTES = 2 << 30                # keys and values that `_attention_after` joins at a time
 
     def __init__(self, *a, use_mfma: bool = True, long_context: bool = False, **kw):
         super().__init__(*a, **kw)
@@ -383,6 +384,25 @@ class HipLlamaStep(TorchLlamaStep):
     def _attention(self, q, k, v, key_mask=None):
         from . import ops
         return ops.attention(q, k, v, key_mask=key_mask, scale=self.scale)
+
+    def _attention_after(self, parts, q, k, v) -> torch.Tensor:
+        """Attention of sequences [Z, L, heads, hd] that continue others: each over [every part ; its own k, v].  parts:
+        (k, v, which) each, k and v [rows, positions, kv_heads, hd], `which` [Z] the row that a sequence continues, None
+        where there is one row for all.  The joined keys and values are a copy for each sequence, made for as many
+        sequences at a time as JOIN_BYTES hold (one at least)."""
+        Z, kv_bytes = q.shape[0], 2 * k.shape[2] * k.shape[3] * k.element_size()
+        positions = k.shape[1] + sum(p[0].shape[1] for p in parts)
+        n = max(1, self.JOIN_BYTES // max(1, positions * kv_bytes))
+
+        def some(z0, z1):
+            rows = [[x.expand(z1 - z0, -1, -1, -1) if which is None else x.index_select(0, which[z0:z1]) for x in kv]
+                    for *kv, which in parts]
+            joined = (torch.cat([r[i] for r in rows] + [x[z0:z1]], dim=1) for i, x in ((0, k), (1, v)))
+            return self._attention(q[z0:z1], *joined)
+
+        if n >= Z:
+            return some(0, Z)
+        return torch.cat([some(z, min(z + n, Z)) for z in range(0, Z, n)])
 
     @torch.no_grad()
     def encode_context(self, context: torch.Tensor, beam: int, max_new_tokens: int,
@@ -443,10 +463,10 @@ class HipLlamaStep(TorchLlamaStep):
             self.kp.append(own[0])
             self.vp.append(own[1])
             self.levels.append([own] if self.S else [])
-            if self.P:
-                self.levels[l].insert(0, (kpre[l].transpose(1, 2), vpre[l].transpose(1, 2)))
-                k, v = (torch.cat((a.expand(self.N, -1, -1, -1), b), dim=1) for a, b in ((kpre[l], k), (vpre[l], v)))
-            return self._attention(q, k, v)
+            if not self.P:
+                return self._attention(q, k, v)
+            self.levels[l].insert(0, (kpre[l].transpose(1, 2), vpre[l].transpose(1, 2)))
+            return self._attention_after([(kpre[l], vpre[l], None)], q, k, v)
 
         if prefix is not None and prefix.shape[0]:
             self._layers(prefix[None], 0, keep)
@@ -465,14 +485,8 @@ class HipLlamaStep(TorchLlamaStep):
 
         def attend(l, q, k, v):
             # [prefix ; the utterance's context ; the sequence]
-            levels = [x for x in self.levels[l]]
-            parts = []
-            if self.P:
-                parts.append([x.transpose(1, 2).expand(M, -1, -1, -1) for x in levels.pop(0)])
-            if levels:
-                parts.append([x.transpose(1, 2).index_select(0, utt) for x in levels[0]])
-            k, v = (torch.cat([p[i] for p in parts] + [x], dim=1) for i, x in ((0, k), (1, v)))
-            return self._attention(q, k, v)
+            which = ([None] if self.P else []) + [utt]
+            return self._attention_after([(*(x.transpose(1, 2) for x in kv), w) for kv, w in zip(self.levels[l], which)], q, k, v)
 
         h = self._layers(F.embedding(seq[:, :L - 1], self.w["char_embed"]), self.P + self.S, attend)
         return F.linear(h, self.w["lm_head.w"], self.w["lm_head.b"]).float()

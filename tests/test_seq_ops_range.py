@@ -184,6 +184,36 @@ def test_what_rows_without_keys_hold_takes_no_part(dtype, Z, L, KVH, G, D, pad):
     assert not bool(grads[0][rows.cuda()].any())
 
 
+# ---------------------------------------------------------------------- a shared prompt joined to many sequences
+@pytest.mark.gpu
+def test_sequences_that_share_a_prompt_are_joined_a_few_at_a_time():
+    """Teacher-forced rows and contexts behind a prompt: the copies of the prompt's keys and values stay within
+    JOIN_BYTES (and what one sequence needs), and the rows are the same bits whatever that is."""
+    from tests.test_ar_head import _small_dims, _small_head
+    g = _gen(21)
+    dims = _small_dims(layers=1, heads=8, kv_heads=8, head_dim=64)
+    seq, lens = torch.randint(0, 37, (9, 7), generator=g), torch.full((9,), 7)
+    prefix, ctx = torch.randn(6, dims.hidden, generator=g), torch.randn(5, 9, dims.hidden, generator=g)
+    got = []
+    for room in (None, 1, 100_000):                             # all at once, one by one, four by four (22 positions of 4 KiB)
+        head = _small_head("HipLlamaStep", dims, "cuda")
+        head.JOIN_BYTES = room or head.JOIN_BYTES
+        head.encode_context(ctx, 2, 3, prefix=prefix)
+        got.append((head.teacher_logits(seq, lens), head.teacher_logits(seq, lens, torch.randint(0, 5, (9,), generator=_gen(1)))))
+    assert all(torch.equal(a, b) for other in got[1:] for a, b in zip(other, got[0]))
+    assert not torch.equal(*got[0])
+    # 64 sequences behind 8192 positions: 1 GiB of copies in bf16
+    head = _small_head("HipLlamaStep", dims, "cuda", torch.bfloat16)
+    head.JOIN_BYTES = 64 << 20
+    seq, lens = torch.randint(0, 37, (64, 5), generator=g), torch.full((64,), 5)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    head.encode_context(torch.randn(64, 2, dims.hidden, generator=g), 2, 3, prefix=torch.randn(8192, dims.hidden, generator=g))
+    head.teacher_logits(seq, lens)
+    assert torch.cuda.max_memory_allocated() - before < 512 << 20
+
+
 # ---------------------------------------------------------------------- assembly leaves m0 alone
 def test_assembly_restores_m0():
     """m0 is the compiler's (it keeps the index of a register array there, for instance, and cannot be told that a statement
