@@ -6,6 +6,7 @@ that results are reproducible on the host.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -41,7 +42,14 @@ def _older(so: Path, sources) -> bool:
 
 
 def stale() -> bool:
-    return _older(SO, [CSRC / s for s in SOURCES] + HEADERS)
+    """Whether a source, a header or the flags (this file) changed since libnsdecode.so was built."""
+    return _older(SO, [CSRC / s for s in SOURCES] + HEADERS + [Path(__file__)])
+
+
+def torch_side_stale() -> bool:
+    """The same of _nsd_torch.so, which also belongs to the torch that it was built against."""
+    torch_version = Path(importlib.util.find_spec("torch").origin).parent / "version.py"
+    return _older(TORCH_SO, [TORCH_SOURCE, API, Path(__file__), torch_version])
 
 
 def _run(cmd, verbose: bool) -> None:
@@ -73,7 +81,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     jobs = []
     if force or stale():
         jobs.append(_build_kernels)
-    if force or _older(TORCH_SO, [TORCH_SOURCE, API]):
+    if force or torch_side_stale():
         jobs.append(_build_torch_side)
     with ThreadPoolExecutor(2) as pool:
         list(pool.map(lambda job: job(verbose), jobs))
