@@ -149,8 +149,8 @@ NSD_D double nsd_xchg_f64(double v)
     return __longlong_as_double((long long)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo));
 }
 
-// Two exponentials at once with the packed fp32 instructions (v_pk_mul/fma/add_f32 are IEEE per element,
-// so each half has the bits of nsd_det_expf).
+// Two exponentials at once, each half with the bits of nsd_det_expf.  (The library is compiled without packed fp32
+// instructions, so these are two independent chains of scalar ones.)
 typedef float nsd_f2 __attribute__((ext_vector_type(2)));
 
 NSD_D nsd_f2 nsd_det_expf2(nsd_f2 d)

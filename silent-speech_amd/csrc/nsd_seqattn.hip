@@ -10,7 +10,11 @@
 // halves, and the probabilities already lie as the B operand of O^T = V^T P^T - slot j of lane half h is key
 // 8 (j / 4) + 4 h + j % 4 of 16, and the V^T operand is read from LDS in that same order of keys (ds_read_b64_tr_b16
 // transposes the row-major tile on the way).  Scores, probabilities and sums are fp32; probabilities and their
-// gradients are rounded to bf16 only where they enter a bf16 product.
+// gradients are rounded to bf16 only where they enter a bf16 product.  That takes the error of a result against 64 bits from
+// 1.65e-3 of its size (its own rounding) to 1.9e-3, and of a gradient to 2.4e-3.  A second product with what the rounding
+// left (rest_frag) takes it back for a third to a half more matrix instructions: done in the backward pass where a launch
+// waits on latencies and has them free (FINE), so the last bits of a sequence's gradients depend on how many sequences share
+// its batch.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "nsd_device.h"
@@ -214,7 +218,8 @@ NSD_D uint32_t rest4(float a, float b, float c, float d)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint32_t hi = i ? u & 0xffff0000u : u << 16;
-            // 2^15 / 2^exponent; a value below 2^-111 has no rest
+            // 2^15 / 2^exponent, of 2^-111 for what is below it: rest_dot then takes less of the rest than there was, by 2^-120
+            // at most
             const float inv = __uint_as_float(max(0x7f000000u + (15u << 23) - max(hi & 0x7f800000u, 16u << 23), 0u));
             r = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_fmaf(v[j + i] - __uint_as_float(hi), inv, 128.0f), j + i, r);
         }
@@ -1122,8 +1127,8 @@ void split_walk(Plan &p, int64_t wgs, int64_t steps, int64_t room, int64_t least
 // dimensions up to 64 and 128; 1600 with few rows) whether one workgroup waits for it on a CU or two, an fp32 tile 3100
 // and 5200, with two workgroups 1.5 and 2 times that; the join takes 3 us and 33 ns for each share of 128 rows.  A beam step
 // over one prefix, 8 kv heads, as many workgroups as there is room for against this: 1024 hypotheses, 24 heads of 128: 512
-// positions 54 and 44 us, 2048 77 and 77, 8192 170 and 170 (2048 without a split: 91); 512 with 16 heads of 64: 26 and 25,
-// 41 and 36, 56 and 56.
+// positions 55 and 44 us, 2048 77 and 77, 8192 170 and 171 (2048 without a split: 91); 512 with 16 heads of 64: 37 and 25,
+// 41 and 37, 56 and 56.
 void split_keys(Plan &p, int64_t wgs, int64_t steps, int DP, int dtype)
 {
     const bool wide = DP == 128;

@@ -6,9 +6,11 @@ for prompts and scored candidates, and for beam steps over long prefixes.
     add_rms_norm(x, delta, w)           residual add + RMSNorm, differentiable           nsd_add_rmsnorm, nsd_add_rmsnorm_bwd
 
 Device tensors in float32 or bfloat16; there is no CPU fall-back.  Kernels run on the current stream of the tensors'
-device; scratch comes from torch's allocator, call by call.  Same arguments, same bits.  Arguments are checked and the
+device; scratch comes from torch's allocator, call by call.  Same arguments, same bits; the order of sums, and with it the
+last bits, follows from all sizes of a call, the batch's among them.  Arguments are checked and the
 autograd nodes live in csrc/nsd_torch.cpp: ValueError and TypeError for arguments, NsdError for what the library
 refuses.  Derivatives are reverse-mode only: a tensor with a forward-mode tangent (torch.autograd.forward_ad) is refused.
+A backward pass is captured into a graph from leaves made inside the capture (x.detach().requires_grad_()).
 """
 from __future__ import annotations
 
@@ -52,7 +54,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     i // (heads // kv_heads)); hd a multiple of 8 up to 128; any strides.  causal: query i sees keys j <= i + Lk - Lq.
     key_mask [Z, Lk] bool (or uint8): keys that are False are seen by no query, whatever they hold.  A query that sees
     no key gives zeros and has no part in any gradient, whatever it and its row of the output's gradient hold.  scale > 0,
-    default 1 / sqrt(hd).  Returns [Z, Lq, heads, hd]."""
+    default 1 / sqrt(hd).  Returns [Z, Lq, heads, hd].
+
+    bfloat16: softmax and sums are float32; probabilities and their gradients are rounded to bfloat16 where they enter a
+    product, in small launches to 16 bits (a relative error of 1.9e-3 of a result and up to 2.4e-3 of a gradient, where
+    their own rounding makes 1.7e-3)."""
     return (_torch_side or load()).attention(q, k, v, causal, key_mask, scale)
 
 
@@ -72,7 +78,9 @@ def shared_prefix_attention(q: torch.Tensor, prefixes: Sequence, kgen: torch.Ten
 
 def add_rms_norm(x: torch.Tensor, delta: Optional[torch.Tensor], w: torch.Tensor, eps: float = 1e-5):
     """(x_out, h): x_out = x + delta (x itself where delta is None), h = w * x_out * rsqrt(mean(x_out^2) + eps) over
-    the last axis, both in the tensors' type, differentiable (once) in x, delta and w.
+    the last axis, both in the tensors' type, differentiable (once) in x, delta and w.  In bfloat16 the normed row is
+    rounded before w is applied, and the product again, as LlamaRMSNorm does.  The rows' mean squares have to be inside
+    float32.
 
     x, delta [..., hidden], w [hidden]; hidden a multiple of 4 (float32) or 8 (bfloat16)."""
     return (_torch_side or load()).add_rms_norm(x, delta, w, eps)
