@@ -5,6 +5,8 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/custom_class.h>
 #include <torch/extension.h>
 #include <cmath>
 #include <string>
@@ -103,15 +105,38 @@ void strides(int64_t (&s)[3], const Tensor &t, int a, int b, int c)
     for (int i = 0; i < 3; ++i) s[i] = t.size(axis[i]) > 1 ? t.stride(axis[i]) : 0;
 }
 
+// What a node keeps for its backward pass beside tensors: a number and a truth value of the call, and the way to its
+// arguments' own nodes.
+struct Kept : torch::CustomClassHolder {
+    double number;
+    bool flag;
+    torch::autograd::edge_list edges;
+};
+template <class... Args> void keep(AutogradContext *ctx, double number, bool flag, const Args &...args)
+{
+    auto k = c10::make_intrusive<Kept>();
+    k->number = number;
+    k->flag = flag;
+    k->edges = torch::autograd::collect_next_edges(args...);
+    ctx->saved_data["kept"] = at::IValue::make_capsule(std::move(k));
+}
+const Kept &kept(AutogradContext *ctx) { return *static_cast<const Kept *>(ctx->saved_data["kept"].toCapsule().get()); }
+
 // Gradients computed by these nodes are not differentiable themselves: where a graph of them is asked for, they carry a
-// node that raises when it is walked.
-variable_list once(variable_list grads, const char *name)
+// node that raises when it is walked.  It leads on to what they depend on, the operator's arguments and the gradients that
+// came in: a walk to one of those that met no node on its way would take them for independent of it, and give zeros.
+variable_list once(AutogradContext *ctx, const variable_list &came_in, variable_list grads, const char *name)
 {
     if (!at::GradMode::is_enabled()) return grads;
-    auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " is differentiable once", (int)grads.size());
+    auto edges = kept(ctx).edges;
+    for (auto &e : torch::autograd::collect_next_edges(came_in)) edges.push_back(std::move(e));
+    const auto error = std::make_shared<torch::autograd::Error>(std::string(name) + " is differentiable once", std::move(edges));
     for (auto &g : grads)
-        if (g.defined()) g = g.detach().requires_grad_();
-    return (*error)(std::move(grads));
+        if (g.defined()) {
+            g = g.detach();
+            torch::autograd::set_history(g, error);
+        }
+    return grads;
 }
 
 // ---------------------------------------------------------------------- attention of whole sequences
@@ -155,8 +180,7 @@ struct Attention : torch::autograd::Function<Attention> {
         Tensor lse, rest;
         Tensor out = attn_fwd(q, k, v, mask, causal, scale, &lse, &rest);
         ctx->save_for_backward({q, k, v, mask, out, lse, rest});
-        ctx->saved_data["causal"] = causal;
-        ctx->saved_data["scale"] = scale;
+        keep(ctx, scale, causal, q0, k0, v0);
         return out;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
@@ -168,7 +192,7 @@ struct Attention : torch::autograd::Function<Attention> {
         {
             const c10::DeviceGuard guard(q.device());
             const at::AutoGradMode no_grad(false);
-            const NsdSeqAttn p = seq_of(q, k, v, mask, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
+            const NsdSeqAttn p = seq_of(q, k, v, mask, kept(ctx).flag, kept(ctx).number);
             const auto opt = q.options().requires_grad(false);
             const Tensor dout = packed(grads[0]);
             d[0] = at::empty(q.sizes(), opt);
@@ -179,7 +203,7 @@ struct Attention : torch::autograd::Function<Attention> {
             check(lib.attn_bwd(ptr(q), ptr(k), ptr(v), ptr(out), (const float *)ptr(lse), (const uint8_t *)ptr(rest), ptr(dout), &p,
                                ptr(d[0]), ptr(d[1]), ptr(d[2]), ptr(ws), n, stream_of(q)), "nsd_attn_bwd");
         }
-        return once(std::move(d), "attention");
+        return once(ctx, grads, std::move(d), "attention");
     }
 };
 
@@ -314,8 +338,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
         const Tensor xc = packed(x), dc = delta.defined() ? packed(delta) : Tensor(), wc = packed(w);
         auto [x_out, h] = norm_fwd(x, xc, dc, wc, eps);
         ctx->save_for_backward({delta.defined() ? x_out : xc, wc});
-        ctx->saved_data["eps"] = eps;
-        ctx->saved_data["delta"] = delta.defined();
+        keep(ctx, eps, delta.defined(), x, delta, w);
         return {x_out, h};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
@@ -323,7 +346,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1];
         no_tangents("add_rms_norm's gradient", {&x, &w, &grads[0], &grads[1]});
-        const bool delta = ctx->saved_data["delta"].toBool();
+        const bool delta = kept(ctx).flag;
         const bool want_w = ctx->needs_input_grad(delta ? 2 : 1);   // (counts the tensors among the inputs)
         variable_list d(4);
         {
@@ -341,14 +364,15 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
                 if (want_w) dw = at::empty(w.sizes(), opt);
                 const int64_t n = want_w ? lib.add_rmsnorm_bwd_workspace((int)rows, (int)hidden) : 0;
                 const Tensor ws = scratch(n, x);
-                check(lib.add_rmsnorm_bwd(ptr(x), ptr(w), ptr(dh), ptr(go), (float)ctx->saved_data["eps"].toDouble(), (int)rows, (int)hidden,
+                check(lib.add_rmsnorm_bwd(ptr(x), ptr(w), ptr(dh), ptr(go), (float)kept(ctx).number, (int)rows, (int)hidden,
                                           x.scalar_type() == at::kBFloat16, ptr(dx), ptr(dw), ptr(ws), n, stream_of(x)), "nsd_add_rmsnorm_bwd");
             }
             if (ctx->needs_input_grad(0)) d[0] = dx;
             if (delta && ctx->needs_input_grad(1)) d[1] = dx;
             d[2] = dw;
         }
-        return once(std::move(d), "add_rms_norm");
+        if (!grads[1].defined()) return d;                      // (what only passed through keeps its own history)
+        return once(ctx, grads, std::move(d), "add_rms_norm");
     }
 };
 

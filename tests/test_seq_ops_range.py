@@ -93,6 +93,38 @@ def test_forward_mode_is_refused_on_the_device(grad):
     assert ops.attention(q, q, q).shape == q.shape
 
 
+@pytest.mark.gpu
+def test_gradients_of_gradients_raise_whatever_they_are_taken_for():
+    """Also where torch may leave out what a result does not depend on (allow_unused, its functional Hessian): a gradient is
+    not independent of the arguments that it was computed from, nor of the gradient that came in."""
+    from silent_speech_amd import ops
+    g = _gen(4)
+    rnd = lambda *s: torch.randn(*s, generator=g).cuda().requires_grad_()   # noqa: E731
+    def strided(x):                                                         # noqa: E306
+        return torch.stack((x, x), -1)[..., 0]                             # (copied inside)
+    for form in (lambda x: x, strided):
+        q, k, v, do = rnd(1, 9, 4, 32), rnd(1, 9, 2, 32), rnd(1, 9, 2, 32), rnd(1, 9, 4, 32)
+        out = ops.attention(*(form(x) for x in (q, k, v)))
+        grads = torch.autograd.grad(out, (q, k, v), do, create_graph=True)
+        for d in grads:
+            for x in (q, k, v, do):
+                with pytest.raises(RuntimeError, match="differentiable once"):
+                    torch.autograd.grad(d.sum(), x, retain_graph=True, allow_unused=True)
+        x, delta, w, go, dh = rnd(3, 32), rnd(3, 32), rnd(32), rnd(3, 32), rnd(3, 32)
+        x_out, h = ops.add_rms_norm(form(x), form(delta), w)
+        grads = torch.autograd.grad((x_out, h), (x, delta, w), (go, dh), create_graph=True)
+        for d in grads:
+            for y in (x, delta, w, go, dh):
+                with pytest.raises(RuntimeError, match="differentiable once"):
+                    torch.autograd.grad(d.sum(), y, retain_graph=True, allow_unused=True)
+        (dx,) = torch.autograd.grad(ops.add_rms_norm(form(x), form(delta), w)[0], x, go, create_graph=True)
+        (one,) = torch.autograd.grad(dx.sum(), go)                          # the sum's own: what came in
+        assert torch.equal(dx, go) and torch.equal(one, torch.ones_like(go))
+    w = torch.ones(32, device="cuda")
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.functional.hessian(lambda x: ops.add_rms_norm(x, None, w)[1].sum(), torch.randn(2, 32, device="cuda"))
+
+
 # ---------------------------------------------------------------------- shapes that only the gradients refuse
 def test_attention_refuses_before_the_forward_pass_what_its_gradients_refuse():
     from silent_speech_amd import lib, ops
