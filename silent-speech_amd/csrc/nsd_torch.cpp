@@ -86,17 +86,18 @@ Tensor scratch(int64_t bytes, const Tensor &like)
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 bool aligned(const Tensor &t) { return ((uintptr_t)t.data_ptr() & 15) == 0; }
 
-// t, or a copy of it, with consecutive elements in its rows and everything else in steps of 16 bytes
+// t, or a copy of it, with consecutive elements in its rows and everything else in steps of 16 bytes, and with the values
+// themselves in memory (a view may have a sign that is not applied there yet: the imaginary part of a conjugate)
 Tensor in_rows(const Tensor &t)
 {
     const int64_t piece = 16 / t.element_size();
-    bool ok = t.stride(-1) == 1 && aligned(t);
+    bool ok = t.stride(-1) == 1 && !t.is_neg() && aligned(t);
     for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) == 1 || t.stride(i) % piece == 0);
     return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 Tensor packed(const Tensor &t)
 {
-    const Tensor c = t.contiguous();
+    const Tensor c = t.resolve_neg().contiguous();
     return aligned(c) ? c : c.clone();
 }
 void strides(int64_t (&s)[3], const Tensor &t, int a, int b, int c)
@@ -261,7 +262,7 @@ Tensor shared_prefix_attention(const Tensor &q0, const std::vector<std::vector<T
     same_device(name, q0, {&kgen, &vgen, &anc});
     const int dt = same_type(name, q0, {&kgen, &vgen});
     bool grad = q0.requires_grad() || kgen.requires_grad() || vgen.requires_grad();
-    if (!kgen.is_contiguous() || !vgen.is_contiguous() || (anc.defined() && !anc.is_contiguous()))
+    if (!kgen.is_contiguous() || !vgen.is_contiguous() || kgen.is_neg() || vgen.is_neg() || (anc.defined() && !anc.is_contiguous()))
         bad_value(at_ + "the generated cache and its ancestor table are contiguous");
     if (t > 0 && (!anc.defined() || anc.scalar_type() != at::kByte || anc.dim() != 2 || anc.size(0) < t || anc.size(1) != M))
         bad_value(at_ + "anc is uint8 [>= t, M]");

@@ -216,6 +216,37 @@ def test_what_rows_without_keys_hold_takes_no_part(dtype, Z, L, KVH, G, D, pad):
     assert not bool(grads[0][rows.cuda()].any())
 
 
+# ---------------------------------------------------------------------- signs that are not in memory yet
+@pytest.mark.gpu
+def test_views_with_a_sign_of_their_own():
+    from silent_speech_amd import ops
+    g = _gen(6)
+    rnd = lambda *s: torch.randn(*s, generator=g).cuda()        # noqa: E731
+    neg = torch._neg_view                                       # what x.conj().imag is, here with rows in steps of one
+    assert neg(rnd(2)).is_neg() and rnd(2).to(torch.complex64).conj().imag.is_neg()
+    x = [rnd(1, 9, h, 32) for h in (4, 2, 2)]
+    do = rnd(1, 9, 4, 32)
+    for i in range(4):
+        got, want = ([f(y) if j == i else y for j, y in enumerate((*x, do))] for f in (neg, torch.neg))
+        a, b = ([y.detach().requires_grad_() for y in z[:3]] for z in (got, want))
+        oa, ob = ops.attention(*a), ops.attention(*b)
+        assert torch.equal(oa, ob) and torch.equal(ops.attention(*got[:3]), ob)
+        for da, db in zip(torch.autograd.grad(oa, a, got[3]), torch.autograd.grad(ob, b, want[3])):
+            assert torch.equal(da, db)
+    r = [rnd(3, 32), rnd(3, 32), rnd(32)]
+    for i in range(3):
+        got, want = (ops.add_rms_norm(*(f(y) if j == i else y for j, y in enumerate(r))) for f in (neg, torch.neg))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    q, k, v, kg = rnd(4, 4, 32), rnd(1, 2, 5, 32), rnd(1, 2, 5, 32), rnd(1, 4, 2, 32)
+    for i in range(3):
+        got, want = ([f(y) if j == i else y for j, y in enumerate((q, k, v))] for f in (neg, torch.neg))
+        a, b = (ops.shared_prefix_attention(z[0], [tuple(z[1:])], kg, kg, None, 0, 2) for z in (got, want))
+        assert torch.equal(a, b)
+    for bad in ((neg(kg), kg), (kg, neg(kg))):
+        with pytest.raises(ValueError):
+            ops.shared_prefix_attention(q, [(k, v)], *bad, None, 0, 2)
+
+
 # ---------------------------------------------------------------------- a shared prompt joined to many sequences
 @pytest.mark.gpu
 def test_sequences_that_share_a_prompt_are_joined_a_few_at_a_time():
